@@ -159,7 +159,7 @@ def prepare(case, seed):
             flat = torch.cat([t.reshape(g, -1) for layer in nets(case, seed) for t in layer], 1)
             snap = ddrl_amd.PolicySnapshot.shaped(g, d[0], d[-1], d[1:-1], hidden, last, bits=bits)
             snap.load_flat_dev(flat.data_ptr(), flat.shape[1])
-            snap.sync()
+            torch.cuda.synchronize()
         else:
             snap = ddrl_amd.PolicySnapshot.shaped(g, d[0], d[-1], [], hidden, last, bits=bits)
         state["snap"] = snap
