@@ -71,6 +71,26 @@ class EnvVtable(C.Structure):
                 ("apply", APPLY), ("running", FLAG), ("final_state", FLAG), ("next_instance", NEXT), ("dump", DUMP)]
 
 
+class SnapForwardArgs(C.Structure):
+    _fields_ = [("n", C.c_int), ("x", C.c_void_p), ("x_agent", C.c_int64), ("x_row", C.c_int64),
+                ("out", C.c_void_p), ("out_agent", C.c_int64), ("out_row", C.c_int64), ("mask", C.c_void_p), ("stream", C.c_void_p)]
+
+
+class SnapMixtureArgs(C.Structure):
+    _fields_ = [("n", C.c_int), ("top_k", C.c_int), ("x", C.c_void_p), ("x_row", C.c_int64),
+                ("router_w", C.c_void_p), ("router_row", C.c_int64), ("router_b", C.c_void_p),
+                ("allowed", C.c_void_p), ("allowed_row", C.c_int64), ("out", C.c_void_p), ("out_row", C.c_int64),
+                ("idx", C.c_void_p), ("prob", C.c_void_p), ("y", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p)]
+
+
+class SnapMixtureGradArgs(C.Structure):
+    _fields_ = [("n", C.c_int), ("top_k", C.c_int), ("x", C.c_void_p), ("x_row", C.c_int64),
+                ("idx", C.c_void_p), ("prob", C.c_void_p), ("y", C.c_void_p), ("dout", C.c_void_p), ("dout_row", C.c_int64),
+                ("d_router_w", C.c_void_p), ("d_router_row", C.c_int64), ("d_router_b", C.c_void_p), ("dy", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p)]
+
+
 # every symbol include/ddrl_pop.h declares: (name, restype, argtypes)
 _vp, _i, _cp = C.c_void_p, C.c_int, C.c_char_p
 SYMBOLS = [
@@ -187,6 +207,20 @@ SYMBOLS = [
     ("ddrl_nfac_update", _i, [_vp, _vp]),
     ("ddrl_nfac_last", _i, [_vp, _vp, _vp, _vp]),
     ("ddrl_nfac_learn_batch_lw", _i, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, _vp]),
+    ("ddrl_snap_create", _i, [_i, _i, _i, _vp, _i, _i, _i, _i, _i, C.POINTER(_vp)]),
+    ("ddrl_snap_create_from", _i, [_vp, _i, _i, C.POINTER(_vp)]),
+    ("ddrl_snap_destroy", _i, [_vp]),
+    ("ddrl_snap_shape", _i, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    ("ddrl_snap_load", _i, [_vp, _vp, _i, _vp]),
+    ("ddrl_snap_load_flat_dev", _i, [_vp, _vp, C.c_int64, _vp]),
+    ("ddrl_snap_get_weights", _i, [_vp, _vp]),
+    ("ddrl_snap_forward_dev", _i, [_vp, C.POINTER(SnapForwardArgs)]),
+    ("ddrl_snap_forward", _i, [_vp, _i, _vp, _vp]),
+    ("ddrl_snap_mixture_workspace", _i, [_vp, _i, _i, C.POINTER(C.c_size_t)]),
+    ("ddrl_snap_mixture_dev", _i, [_vp, C.POINTER(SnapMixtureArgs)]),
+    ("ddrl_snap_mixture", _i, [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    ("ddrl_snap_mixture_grad_workspace", _i, [_vp, _i, _i, C.POINTER(C.c_size_t)]),
+    ("ddrl_snap_mixture_grad_dev", _i, [_vp, C.POINTER(SnapMixtureGradArgs)]),
     ("ddrl_cmaes_create", _i, [_i, _vp, _vp, C.c_long, _i, _i, C.POINTER(_vp)]),
     ("ddrl_cmaes_destroy", _i, [_vp]),
     ("ddrl_cmaes_sample", _i, [_vp]),

@@ -552,6 +552,106 @@ int ddrl_sim_run(ddrl_sim_t *s);
 /* Simulator::run_episode (:139-208) for all G (agent, environment) pairs */
 int ddrl_sim_run_episode(ddrl_sim_t *s, int learning, long lepisode, long tepisode);
 
+/* ------------------------------------------------------------------------------------------------
+ * Served snapshots (no counterpart in the reference, which answers with the net it trains): a copy of one net of every agent
+ * of a population in a layout made for answering, its weights in 32 bits or in 4, and two ways to ask it: every agent for
+ * its own states (ddrl_snap_forward*, what ddrl_pop_infer / ddrl_pop_forward_batch do on the live nets), or all agents
+ * together as the experts of a mixture behind a linear router (ddrl_snap_mixture*), whose gradient in the router's
+ * parameters is ddrl_snap_mixture_grad_dev.
+ *
+ * 4-bit weights are the OCP MX format (MXFP4): a weight is one of +-{0, .5, 1, 1.5, 2, 3, 4, 6} (E2M1) times a power of two
+ * that 32 consecutive inputs of one output share (the last block of a row may be shorter).  Loading takes the least power
+ * of two that keeps the block's largest magnitude within 6 and rounds to the nearest, halves to the even code.  A block
+ * whose largest magnitude is under 2^-118 becomes zeros; an output with a weight that is not finite, or of magnitude 2^126
+ * or more, answers NaN.  Biases stay in 32 bits.  Activations and sums are 32-bit in both formats.
+ *
+ * A snapshot is not written by the calls that ask it, and they keep nothing in it: the _dev calls take the stream to run on
+ * and, where they need one, a workspace of the caller's.  They may be captured into a HIP graph, and calls on several
+ * streams or from several host threads may overlap as long as their outputs and workspaces do not.  (ddrl_snap_load,
+ * ddrl_snap_load_flat_dev and ddrl_snap_destroy write the snapshot: the caller keeps them apart from the calls that ask it.)
+ * Pointers of the _dev calls are device memory of the snapshot's GPU (DDRL_EINVAL for NULL and for pointers that are not
+ * aligned to their type, not for other wrong ones); the current device of the calling thread is left as it was.  Strides
+ * count elements; -1 = rows packed one after the other; outputs' rows must not overlap each other, nor any input.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct ddrl_snap ddrl_snap_t;
+#define DDRL_SNAP_MAX_TOP_K 8
+
+/* an empty snapshot (zero weights) for nets in_dim - hidden[0] - .. - out_dim: dimensions 1..1024, 0..3 hidden layers;
+ * hidden_layer_type 0..3, output_layer_type 0..3 (0 linear, 1 leaky-ReLU(0.01), 2 tanh, 3 ReLU); bits 32 or 4 */
+int ddrl_snap_create(int n_agents, int in_dim, int out_dim, const int *hidden, int n_hidden, int hidden_layer_type,
+                     int output_layer_type, int bits, int device, ddrl_snap_t **out);
+/* the same with the dimensions, activations and GPU of a population's net, loaded from it */
+int ddrl_snap_create_from(ddrl_pop_t *h, int net, int bits, ddrl_snap_t **out);
+int ddrl_snap_destroy(ddrl_snap_t *s);
+/* any pointer may be NULL; n_params: per agent, in the flat order */
+int ddrl_snap_shape(ddrl_snap_t *s, int *n_agents, int *in_dim, int *out_dim, int *bits, int *n_params);
+/* takes the net's parameters as they are after everything the population has been asked for (waits for it on the host) and
+ * lays them out on `stream`; later updates of the population wait for that on the GPU.  The net must have the snapshot's
+ * dimensions and activations and be on its GPU; nets with BatchNorm towers and populations with developmental gates in
+ * force are refused (DDRL_EINVAL, DDRL_ESTATE: a snapshot holds InnerProducts only), so is a capturing stream (DDRL_ESTATE). */
+int ddrl_snap_load(ddrl_snap_t *s, ddrl_pop_t *h, int net, void *stream);
+/* the same from fp32 rows [n_agents x ld] in the flat order, as ddrl_pop_load_flat_dev (ld == 0: one row for every agent) */
+int ddrl_snap_load_flat_dev(ddrl_snap_t *s, const float *d_flat, int64_t ld, void *stream);
+/* what the stored weights stand for, [n_agents x n_params], flat order; waits for the whole GPU first */
+int ddrl_snap_get_weights(ddrl_snap_t *s, double *flat);
+
+/* every agent's net on n rows: x [n_agents x n x in_dim] -> out [n_agents x n x out_dim] */
+typedef struct {
+  int n;                                   /* rows per agent, >= 0 */
+  const float *x;
+  int64_t x_agent, x_row;                  /* x_agent 0: all agents read the same n rows; x_row 0: an agent's rows are one row */
+  float *out;
+  int64_t out_agent, out_row;
+  const uint8_t *mask;                     /* [n_agents] or NULL; an agent with mask 0 is skipped, its rows of out stay as they were */
+  void *stream;                            /* hipStream_t; NULL = the default stream of the snapshot's GPU */
+} ddrl_snap_forward_args;
+int ddrl_snap_forward_dev(ddrl_snap_t *s, const ddrl_snap_forward_args *a);
+/* host buffers, packed; returns when `out` holds the answer */
+int ddrl_snap_forward(ddrl_snap_t *s, int n, const float *x, float *out);
+
+/* A mixture of the snapshot's nets: row t of x goes to the top_k agents with the largest logits
+ *     l[t, g] = sum_i x[t, i] router_w[g, i] + router_b[g]
+ * among the allowed ones, the lower index first among equals (logits are summed in 64 bits, so that a pick does not hang on
+ * the order of a sum; NaN counts as larger than any number, -infinity as not allowed), and
+ *     prob[t, :] = softmax over the picked logits,   out[t] = sum_j prob[t, j] net_{idx[t, j]}(x[t]).
+ * Where fewer than top_k are left, the last places of idx hold -1, of prob and y 0; a row with none has out = 0. */
+typedef struct {
+  int n, top_k;                            /* rows >= 0; 1 <= top_k <= min(DDRL_SNAP_MAX_TOP_K, n_agents) */
+  const float *x; int64_t x_row;           /* [n x in_dim] */
+  const float *router_w; int64_t router_row;   /* [n_agents x in_dim] */
+  const float *router_b;                   /* [n_agents] or NULL */
+  const uint8_t *allowed; int64_t allowed_row; /* [n x n_agents], 0 = barred; allowed_row 0: one row for all; NULL: all allowed */
+  float *out; int64_t out_row;             /* [n x out_dim] */
+  int32_t *idx; float *prob; float *y;     /* [n x top_k], [n x top_k], [n x top_k x out_dim], packed; each may be NULL */
+  void *workspace; size_t workspace_bytes; /* ddrl_snap_mixture_workspace() bytes, 16-byte aligned; contents do not matter */
+  void *stream;
+} ddrl_snap_mixture_args;
+int ddrl_snap_mixture_workspace(ddrl_snap_t *s, int n, int top_k, size_t *bytes);
+int ddrl_snap_mixture_dev(ddrl_snap_t *s, const ddrl_snap_mixture_args *a);
+/* host buffers, packed; router_b, allowed, idx, prob may be NULL; returns when the answer is there */
+int ddrl_snap_mixture(ddrl_snap_t *s, int n, int top_k, const float *x, const float *router_w, const float *router_b,
+                      const uint8_t *allowed, float *out, int32_t *idx, float *prob);
+
+/* The mixture's gradient for the nets held fixed: from dout = dL/dout [n x out_dim] and what the mixture gave (idx, prob, y)
+ *     dlogit[t, j] = prob[t, j] (dout[t] . y[t, j] - sum_i prob[t, i] dout[t] . y[t, i])
+ *     d_router_w[g, :] = sum over the places (t, j) with idx[t, j] = g of dlogit[t, j] x[t],   d_router_b[g] = sum of dlogit[t, j]
+ *     dy[t, j] = prob[t, j] dout[t]         (dL/dy, for whoever goes on into the nets)
+ * summed in the order of t: the same bits every time.  Places whose idx is outside 0..n_agents-1 add nothing and get dy = 0.
+ * The gradients are written, not added to; a net nobody picked gets zeros. */
+typedef struct {
+  int n, top_k;
+  const float *x; int64_t x_row;
+  const int32_t *idx; const float *prob; const float *y;     /* packed, as the mixture gives them */
+  const float *dout; int64_t dout_row;
+  float *d_router_w; int64_t d_router_row; /* [n_agents x in_dim] */
+  float *d_router_b;                       /* [n_agents] or NULL */
+  float *dy;                               /* [n x top_k x out_dim], packed, or NULL */
+  void *workspace; size_t workspace_bytes; /* ddrl_snap_mixture_grad_workspace() bytes, 16-byte aligned */
+  void *stream;
+} ddrl_snap_mixture_grad_args;
+int ddrl_snap_mixture_grad_workspace(ddrl_snap_t *s, int n, int top_k, size_t *bytes);
+int ddrl_snap_mixture_grad_dev(ddrl_snap_t *s, const ddrl_snap_mixture_grad_args *a);
+
 /* Measurement hooks (no counterpart in the reference, which only records total wall minutes,
  * common/include/arch/Simulator.hpp:127): with profiling on, every ddrl_pop_ddpg_update() brackets
  * its update kernel with HIP events on the handle's stream; ddrl_pop_profile_read() synchronises and
