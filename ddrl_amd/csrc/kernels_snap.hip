@@ -3,6 +3,7 @@
 #include "pop_internal.h"
 #include "snap_internal.h"
 #include <math.h>
+#include <type_traits>
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -11,19 +12,26 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// a run-time index into a by-value kernel argument makes the compiler copy the argument to scratch: select instead
-template <class T>
-__device__ __forceinline__ T pick(const T (&v)[SNAP_MAXL], int l) {
-  T r = v[0];
-#pragma unroll
-  for (int i = 1; i < SNAP_MAXL; ++i) r = l == i ? v[i] + 0 : r;       // (a value: of two lvalues ?: would select the address)
-  return r;
+// The kernels' first argument in the kernel-argument memory itself: a layer is one scalar load there, whatever its number
+// (a run-time index into the by-value argument would make the compiler copy it to scratch memory)
+typedef const __attribute__((address_space(4))) SnapDesc *DescP;
+#define SNAP_DESC(nd) ((DescP)__builtin_amdgcn_kernarg_segment_ptr())
+struct LayerOf { int in, out, strips, steps, act, code; unsigned off, rec; };
+__device__ __forceinline__ LayerOf layer_of(DescP nd, int l) {
+  const __attribute__((address_space(4))) SnapLayer *y = &nd->lay[l];
+  return LayerOf{y->in, y->out, y->strips, y->steps, y->act, y->code, y->off, y->rec};
 }
 
-__device__ __forceinline__ float snap_act(int t, float x) {
-  if (t == 1) return x > 0.f ? x : 0.01f * x;
+__device__ __forceinline__ float act1(int t, float x) {
   if (t == 2) return tanhf(x);
-  if (t == 3) return x > 0.f ? x : (x != x ? x : 0.f);
+  const float low = t == 1 ? 0.01f * x : t == 0 ? x : x != x ? x : 0.f;
+  return x > 0.f ? x : low;
+}
+__device__ __forceinline__ f32x4 act4(int t, f32x4 x) {           // (one decision for four outputs)
+  if (t == 2) return f32x4{tanhf(x[0]), tanhf(x[1]), tanhf(x[2]), tanhf(x[3])};
+  if (t == 0) return x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = x[j] > 0.f ? x[j] : t == 1 ? 0.01f * x[j] : x[j] != x[j] ? x[j] : 0.f;
   return x;
 }
 
@@ -40,22 +48,25 @@ __device__ __forceinline__ unsigned snap_code(float v) {          // v = w / sca
 }
 
 extern "C" __global__ void __launch_bounds__(256)
-snap_load_kernel(const SnapDesc nd, char *__restrict__ img, const SnapSource src, int all_strips) {
-  const int wave = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+snap_load_kernel(const SnapDesc nd_, const SnapSource src, char *__restrict__ img, int all_strips) {
+  const DescP nd = SNAP_DESC(nd_);
+  const int wave = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   if (wave >= all_strips) return;
   int l = 0, strip = wave;
-  while (strip >= pick(nd.strips, l)) { strip -= pick(nd.strips, l); ++l; }
-  const int K = pick(nd.in, l), N = pick(nd.out, l), n = strip * 16 + r, steps = pick(nd.steps, l);
-  const float *w = src.w + (size_t)blockIdx.x * src.agent + pick(src.offw, l);
-  const float *b = src.w + (size_t)blockIdx.x * src.agent + pick(src.offb, l);
-  char *im = img + (size_t)blockIdx.x * nd.stride;
-  const int kp = pick(src.kp, l);
+  while (strip >= nd->lay[l].strips) { strip -= nd->lay[l].strips; ++l; }
+  const LayerOf y = layer_of(nd, l);
+  const int K = y.in, N = y.out, n = strip * 16 + r, steps = y.steps;
+  const __attribute__((address_space(4))) SnapSource *from = (const __attribute__((address_space(4))) SnapSource *)(nd + 1);
+  const float *w = src.w + (size_t)blockIdx.x * src.agent + from->offw[l];
+  const float *b = src.w + (size_t)blockIdx.x * src.agent + from->offb[l];
+  char *rec = img + (size_t)blockIdx.x * nd->stride + y.off + strip * y.rec;
+  const int kp = from->kp[l];
   auto weight = [&](int k) -> float {
     if (n >= N || k >= K) return 0.f;
     return src.tiled ? w[ddrl_widx(n, k, kp)] : w[(size_t)n * K + k];
   };
   bool bad = false;
-  if (nd.bits == 4) {
+  if (nd->bits == 4) {
     for (int s = 0; s < steps; ++s) {
       float v[8], amax = 0.f;
       bool wild = false;
@@ -77,207 +88,402 @@ snap_load_kernel(const SnapDesc nd, char *__restrict__ img, const SnapSource src
       unsigned c = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) c |= (none ? 0u : snap_code(v[i] * inv)) << (4 * i);
-      *(unsigned *)(im + pick(nd.woff, l) + snap_code_off(steps, strip, s, lane)) = c;
-      if (q == 0) im[pick(nd.soff, l) + snap_scale_off(steps, strip, s, r)] = (char)(none ? 127 : sh + 127);
+      *(unsigned *)(rec + s * 256 + lane * 4) = c;
+      if (q == 0) rec[snap_scale_off(y.code, s, r)] = (char)(none ? 127 : sh + 127);
     }
-    if (q == 0) for (int s = steps; s & 3; ++s) im[pick(nd.soff, l) + snap_scale_off(steps, strip, s, r)] = 127;
+    if (q == 0) for (int s = steps; s & 3; ++s) rec[snap_scale_off(y.code, s, r)] = 127;
   } else {
     for (int s = 0; s < steps; ++s) {
       f32x4 v;
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = weight(16 * s + 4 * q + i);
-      *(f32x4 *)(im + pick(nd.woff, l) + ((size_t)strip * steps + s) * 1024 + lane * 16) = v;
+      *(f32x4 *)(rec + s * 1024 + lane * 16) = v;
     }
   }
-  if (q == 0) ((float *)(im + pick(nd.boff, l)))[n] = n >= N ? 0.f : bad ? __uint_as_float(0x7fc00000u) : b[n];
+  if (q == 0) ((float *)(rec + y.rec - 64))[r] = n >= N ? 0.f : bad ? __uint_as_float(0x7fc00000u) : b[n];
 }
 
 extern "C" hipError_t snap_load_launch(const SnapDesc *nd, char *img, const SnapSource *src, int G, hipStream_t st) {
   int all = 0;
-  for (int l = 0; l < nd->L; ++l) all += nd->strips[l];
-  hipLaunchKernelGGL(snap_load_kernel, dim3(G, (all + 3) / 4), dim3(256), 0, st, *nd, img, *src, all);
+  for (int l = 0; l < nd->L; ++l) all += nd->lay[l].strips;
+  hipLaunchKernelGGL(snap_load_kernel, dim3(G, (all + 3) / 4), dim3(256), 0, st, *nd, *src, img, all);
   return hipGetLastError();
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
-// One net on a tile of rows, by one workgroup: D[16 outputs x 16 rows] += A (weights) B (activations) on the matrix cores, a
-// wave per strip of outputs, activations in LDS between the layers (one barrier a layer).
-//   32 bits: v_mfma_f32_16x16x4_f32.
+// One net on a tile of rows, by one workgroup: D[16 outputs x 16 columns] += A (weights) B (activations) on the matrix cores, a
+// wave MT strips of outputs at a time, activations in LDS between the layers (one barrier a layer).
+//   32 bits: v_mfma_f32_16x16x4_f32; a single row: v_fma_f32 on the lane's own 4 weights, the lanes of an output summed at the
+//            end (the matrix instruction would take 8 times as long for one column of use).
 //    4 bits: v_mfma_f32_16x16x32_bf16.  A weight (2 significant bits times a power of two) is exact in bf16, decoded with its
 //            scale by v_cvt_scalef32_pk_bf16_fp4, two weights an instruction; an activation x is exactly the sum of three
 //            bf16 numbers (x's leading 8 bits, the next 8, the last 8), so three products with fp32 accumulation lose no more
 //            than an fp32 product does, at 5 times the fp32 matrix rate.
-//            PACK (up to 5 rows): the three parts of a row are three columns of ONE matrix instruction, summed over the
-//            columns at the end, instead of three instructions with 16 rows each.
+// R rows of 16 columns: 16 (a column each; 4 bits: three products, one for each part), 4 (4 columns each) or 1 (all 16 columns).
+// With 4 bits and R < 16 the columns 4 t, 4 t + 1, 4 t + 2 are the parts of row t: ONE product, summed over the columns at the
+// end.  And with R < 16 every lane finishes ONE output of the tile (bias, activation, the three parts) instead of a few lanes
+// finishing four: with few rows that, not the product, is most of the instructions.
 // ------------------------------------------------------------------------------------------------------------------------
-struct SnapLds { int second; };       // the inputs of layers 0, 2 lie in the first LDS buffer, those of 1, 3 in the second: where that starts
+struct SnapLds { int second, image; };       // the inputs of layers 0, 2 lie in the first LDS buffer, those of 1, 3 in the second; behind them the image, where it is staged
 
-template <int BITS, int NT, bool PACK>
+template <int BITS, int R, int NT>
 struct SnapShape {
-  static constexpr int T = PACK ? 5 : 16 * NT;                               // rows of a tile
-  static constexpr int ROWS = BITS == 4 ? (PACK ? 15 : 48 * NT) : 16 * NT;   // rows of an LDS buffer
+  static constexpr int T = R * NT;                               // rows of a tile (NT > 1: R = 16)
+  static constexpr int ROWS = BITS == 4 ? 3 * T : T;             // rows of an LDS buffer: 4 bits: the rows' first parts, their second ones, their third
   // a row's stride = 16 (mod 32) bytes, so that the 16 lanes that read 16 bytes of 16 rows at once start on distinct banks
   __host__ __device__ static int ld(int K) { return BITS == 4 ? ddrl_roundup(K, 32) * 2 + 16 : ddrl_roundup(K, 16) * 4 + 16; }
   static int bytes(const SnapDesc &nd, SnapLds &m) {
     int a = 0, b = 0;
-    for (int l = 0; l < nd.L; ++l) { int &w = l & 1 ? b : a; w = ld(nd.d[l]) > w ? ld(nd.d[l]) : w; }
+    for (int l = 0; l < nd.L; ++l) { int &w = l & 1 ? b : a; w = ld(nd.lay[l].in) > w ? ld(nd.lay[l].in) : w; }
     m.second = ROWS * a;
-    return ROWS * (a + b);
+    return m.image = ROWS * (a + b);
   }
 };
 
 __device__ __forceinline__ unsigned short bf_top(float x) { return (unsigned short)(__float_as_uint(x) >> 16); }
-// x = p[0] + p[1] + p[2] exactly (down to 2^-133; an infinity or NaN is all in p[0])
-__device__ __forceinline__ void split3(float x, unsigned short (&p)[3]) {
+// x = p[0] + p[1] + p[2] exactly (down to 2^-133), p[j] the upper half of the word v[j]; an infinity or NaN is all in v[0]
+__device__ __forceinline__ void split3(float x, float (&v)[3]) {
   const float hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-  const bool fin = fabsf(x) < __uint_as_float(0x7f800000u);
-  const float r1 = fin ? x - hi : 0.f, mid = __uint_as_float(__float_as_uint(r1) & 0xffff0000u), lo = r1 - mid;
-  p[0] = x != x ? 0x7fc0 : bf_top(x); p[1] = bf_top(mid); p[2] = bf_top(lo);
+  const float r1 = fabsf(x) < __uint_as_float(0x7f800000u) ? x - hi : 0.f;
+  v[0] = x; v[1] = r1;
+  v[2] = r1 - __uint_as_float(__float_as_uint(r1) & 0xffff0000u);
 }
-// the row of an LDS buffer that holds part p of a tile's row t
-template <int BITS, int NT, bool PACK>
-__device__ __forceinline__ int part_row(int t, int p) { return PACK ? 3 * t + p : p * 16 * NT + t; }
+__device__ __forceinline__ unsigned two_tops(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
 
 // `rows(t)`: where row t of the tile lies, or null; all threads of the workgroup, no barrier inside
-template <int BITS, int NT, bool PACK, class Rows>
+template <int BITS, int R, int NT, class Rows>
 __device__ __forceinline__ void tile_in(int K, char *buf, Rows rows) {
-  using S = SnapShape<BITS, NT, PACK>;
+  using S = SnapShape<BITS, R, NT>;
   const int ld = S::ld(K), Kp = BITS == 4 ? (K + 31) & ~31 : (K + 15) & ~15;
-  for (int i = threadIdx.x; i < S::T * Kp; i += blockDim.x) {
-    const int t = i / Kp, k = i - t * Kp;
+  const int per = Kp <= 32 ? 32 : 64;                      // threads a row
+#pragma unroll 2
+  for (int t = threadIdx.x / per; t < S::T; t += blockDim.x / per) {
     const float *x = rows(t);
-    const float v = x && k < K ? x[k] : 0.f;
-    if (BITS == 4) {
-      unsigned short p[3];
-      split3(v, p);
+#pragma unroll 1
+    for (int k = threadIdx.x & (per - 1); k < Kp; k += per) {
+      float v = x && k < K ? x[k] : 0.f;
+      if (BITS == 4) {
+        v = v != v ? __uint_as_float(0x7fc00000u) : v;     // (a NaN that its upper half alone would not show)
+        float p[3];
+        split3(v, p);
 #pragma unroll
-      for (int j = 0; j < 3; ++j) *(unsigned short *)(buf + part_row<BITS, NT, PACK>(t, j) * ld + k * 2) = p[j];
-    } else *(float *)(buf + t * ld + k * 4) = v;
+        for (int j = 0; j < 3; ++j) *(unsigned short *)(buf + (j * S::T + t) * ld + k * 2) = bf_top(p[j]);
+      } else *(float *)(buf + t * ld + k * 4) = v;
+    }
   }
 }
 
-template <int BITS, int NT, bool PACK, class Out>
-__device__ __forceinline__ void net_tile(const SnapDesc &nd, const SnapLds &m, const char *__restrict__ img, char *lds, Out out) {
-  constexpr int P = BITS == 4 && !PACK ? 3 : 1;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, c = lane & 15, q = lane >> 4;
-  for (int l = 0; l < nd.L; ++l) {
-    const char *xin = lds + (l & 1 ? m.second : 0);
-    char *xout = lds + (l & 1 ? 0 : m.second);
-    const int N = pick(nd.out, l), strips = pick(nd.strips, l), steps = pick(nd.steps, l), ldi = SnapShape<BITS, NT, PACK>::ld(pick(nd.in, l));
-    const bool last = l == nd.L - 1;
-    const int ldo = SnapShape<BITS, NT, PACK>::ld(N), act = last ? nd.oact : nd.hact;
-    const char *wl = img + pick(nd.woff, l), *sl = img + pick(nd.soff, l);
-    const float *bl = (const float *)(img + pick(nd.boff, l));
-    for (int s = wave; s < strips; s += waves) {
-      f32x4 acc[NT][P];
+// The barrier between layers: LDS is handed over, the weights already asked for stay in flight across it
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// the value of lane L of the own quad
+template <int L>
+__device__ __forceinline__ float quad_lane(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), L * 0x55, 0xf, 0xf, true)); }
+
+// One k-step of MT strips.  `x`: the step's inputs of this lane's row
+template <int BITS, int R, int NT, int MT, class W>
+__device__ __forceinline__ void step_multiply(const W (&w)[MT], const unsigned (&sc)[MT], int byte, f32x4 (&acc)[MT][NT], const char *x, int ldi) {
+  if constexpr (BITS == 4) {
+    constexpr int P = R == 16 ? 3 : 1;
+    bf16x8 v[NT][P];
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int p = 0; p < P; ++p) acc[i][p] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const f32x4 bias = *(const f32x4 *)(bl + s * 16 + 4 * q);
-      if constexpr (BITS == 4) {
-        const int xrow = PACK ? (c < 15 ? c : 0) : c;
-        auto step = [&](unsigned code, unsigned sb, int at) {
-          const float sc = __uint_as_float(sb << 23);
-          union { bf16x2 h[4]; bf16x8 v; } a;
-          a.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, sc, 0);
-          a.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, sc, 1);
-          a.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, sc, 2);
-          a.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, sc, 3);
+      for (int p = 0; p < P; ++p) v[t][p] = *(const bf16x8 *)(x + (p * R * NT + 16 * t) * ldi);
+    union { bf16x2 h[4]; bf16x8 v; } a[MT];
 #pragma unroll
-          for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-              const bf16x8 b = *(const bf16x8 *)(xin + (p * 16 * NT + 16 * i + xrow) * ldi + at * 64 + q * 16);
-              acc[i][p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b, acc[i][p], 0, 0, 0);
-            }
-        };
-        const char *ws = wl + (size_t)s * steps * 256, *ss = sl + (size_t)s * ((steps + 3) >> 2) * 64 + c * 4;
-        const int full = steps >> 2;
-        for (int b = 0; b < full; ++b) {
-          const u32x4 code = *(const u32x4 *)(ws + b * 1024 + lane * 16);
-          const unsigned sb = *(const unsigned *)(ss + b * 64);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) step(code[j], (sb >> (8 * j)) & 255u, 4 * b + j);
-        }
-        if (steps & 3) {
-          const unsigned sb = *(const unsigned *)(ss + full * 64);
-          for (int j = 0; j < (steps & 3); ++j)
-            step(*(const unsigned *)(ws + full * 1024 + j * 256 + lane * 4), (sb >> (8 * j)) & 255u, 4 * full + j);
-        }
-      } else {
-        const char *ws = wl + (size_t)s * steps * 1024 + lane * 16;
-        for (int b = 0; b < steps; ++b) {
-          const f32x4 a = *(const f32x4 *)(ws + b * 1024);
-#pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            const f32x4 x = *(const f32x4 *)(xin + (16 * i + c) * ldi + b * 64 + q * 16);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], x[j], acc[i][0], 0, 0, 0);
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        f32x4 v = acc[i][0];
-        if constexpr (P == 3) v = (acc[i][2] + acc[i][1]) + v;
-        if constexpr (PACK) {                             // columns 3t, 3t + 1, 3t + 2 are the parts of row t
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int iv = __float_as_int(v[j]);
-            const float m1 = __int_as_float(__builtin_amdgcn_update_dpp(0, iv, 0x101, 0xf, 0xf, true));   // row_shl:1 = column + 1
-            const float m2 = __int_as_float(__builtin_amdgcn_update_dpp(0, iv, 0x102, 0xf, 0xf, true));
-            v[j] = (m2 + m1) + v[j];
-          }
-        }
-        const int t = PACK ? c / 3 : 16 * i + c;
-        const bool mine = !PACK || (c % 3 == 0 && c < 15);
-        const int n0 = s * 16 + 4 * q;
-        float y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = n0 + j < N ? snap_act(act, v[j] + bias[j]) : 0.f;
-        if (last) {
-          if (mine) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) if (n0 + j < N) out(t, n0 + j, y[j]);
-          }
-        } else if (mine) {
-          if constexpr (BITS == 4) {
-            unsigned short p[4][3];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) split3(y[j], p[j]);
-#pragma unroll
-            for (int k = 0; k < 3; ++k) {
-              char *o = xout + part_row<BITS, NT, PACK>(t, k) * ldo + n0 * 2;
-              *(u32x2 *)o = u32x2{p[0][k] | (unsigned)p[1][k] << 16, p[2][k] | (unsigned)p[3][k] << 16};
-              if (s == strips - 1 && (strips & 1)) *(u32x2 *)(o + 32) = u32x2{0u, 0u};      // the next layer's k-steps are 32 wide
-            }
-          } else *(f32x4 *)(xout + t * ldo + n0 * 4) = f32x4{y[0], y[1], y[2], y[3]};
-        }
-      }
+    for (int i = 0; i < MT; ++i) {
+      const float scale = __uint_as_float(((sc[i] >> byte) & 255u) << 23);
+      a[i].h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i], scale, 0);
+      a[i].h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i], scale, 1);
+      a[i].h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i], scale, 2);
+      a[i].h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i], scale, 3);
     }
-    __syncthreads();
+#pragma unroll
+    for (int p = P - 1; p >= 0; --p)                // the small parts first; products of one sum apart from each other
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i].v, v[t][p], acc[i][t], 0, 0, 0);
+  } else if constexpr (R == 1) {
+    const f32x4 v = *(const f32x4 *)x;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][0][j] = fmaf(w[i][j], v[j], acc[i][0][j]);
+  } else {
+    f32x4 v[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) v[t] = *(const f32x4 *)(x + 16 * t * ldi);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i][j], v[t][j], acc[i][t], 0, 0, 0);
   }
 }
+
+// UB k-steps of MT strips, asked for together; those beyond the layer's last step fetch that one again
+template <int BITS, int MT, int UB> struct SnapBlock {
+  using W = std::conditional_t<BITS == 4, unsigned, f32x4>;
+  W w[UB][MT];
+  unsigned sc[(UB + 3) / 4][MT];
+  __device__ __forceinline__ void load(const LayerOf &y, const char *const (&rec)[MT], int b, int lane) {
+    constexpr int SB = BITS == 4 ? 256 : 1024;               // bytes of a step
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+      for (int j = 0; j < UB; ++j) w[j][i] = *(const W *)(rec[i] + min(b + j, y.steps - 1) * SB + lane * sizeof(W));
+      if (BITS == 4) {
+#pragma unroll
+        for (int j = 0; j < UB; j += 4) sc[j / 4][i] = *(const unsigned *)(rec[i] + y.code + min(b + j, (y.steps - 1) & ~3) * 16 + (lane & 15) * 4);
+      }
+    }
+  }
+  // Waits for the block HERE.  Left to itself the compiler waits where it is multiplied, after the next one's loads have gone
+  // out under a condition it cannot count through: it would wait for those too.
+  __device__ __forceinline__ void here() {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+      for (int j = 0; j < UB; ++j) asm volatile("" : "+v"(w[j][i]));
+      if (BITS == 4) {
+#pragma unroll
+        for (int j = 0; j < UB; j += 4) asm volatile("" : "+v"(sc[j / 4][i]));
+      }
+    }
+  }
+};
+
+// What a wave works on: strips s .. s + MT - 1 of layer l
+struct Item { LayerOf y; int l, s; };
+template <int MT>
+__device__ __forceinline__ bool next_item(Item &it, DescP nd, int wave, int waves) {
+  it.s += waves * MT;
+  while (it.s >= it.y.strips) {
+    if (++it.l >= nd->L) return false;
+    it.y = layer_of(nd, it.l);
+    it.s = wave * MT;
+  }
+  return true;
+}
+template <int MT>
+__device__ __forceinline__ void records(const char *(&rec)[MT], const Item &it, const char *img) {
+#pragma unroll
+  for (int i = 0; i < MT; ++i) rec[i] = img + it.y.off + min(it.s + i, it.y.strips - 1) * it.y.rec;
+}
+// The biases a lane needs.  R = 16: of its 4 outputs of every strip; R = 4: of the one of every strip; R = 1: of its one.
+template <int BITS, int R, int MT> struct SnapBias {
+  f32x4 v4[R == 16 ? MT : 1];
+  float v1[R == 4 ? MT : 1];
+  __device__ __forceinline__ void load(const Item &it, const char *const (&rec)[MT], const char *img, int c, int q) {
+    if constexpr (R == 16) { _Pragma("unroll") for (int i = 0; i < MT; ++i) v4[i] = *(const f32x4 *)(rec[i] + it.y.rec - 64 + q * 16); }
+    else if constexpr (R == 4) { _Pragma("unroll") for (int i = 0; i < MT; ++i) v1[i] = *(const float *)(rec[i] + it.y.rec - 64 + (4 * q + (c & 3)) * 4); }
+    else {
+      const int own = BITS == 4 ? (c >> 2) & (MT - 1) : q & (MT - 1), at = BITS == 4 ? 4 * q + (c & 3) : c;
+      v1[0] = *(const float *)(img + it.y.off + min(it.s + own, it.y.strips - 1) * it.y.rec + it.y.rec - 64 + at * 4);
+    }
+  }
+  __device__ __forceinline__ void here() {
+    if constexpr (R == 16) { _Pragma("unroll") for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(v4[i])); }
+    else { _Pragma("unroll") for (int i = 0; i < (R == 4 ? MT : 1); ++i) asm volatile("" : "+v"(v1[i])); }
+  }
+};
+// What is asked for before the inputs are there: the first block of a wave's first strips
+template <int BITS, int R, int MT, int UB> struct SnapAhead { Item it; bool any; SnapBlock<BITS, MT, UB> w; SnapBias<BITS, R, MT> bias; };
+template <int BITS, int R, int MT, int UB>
+__device__ __forceinline__ void ahead_load(SnapAhead<BITS, R, MT, UB> &h, const char *img, int lane) {
+  const char *rec[MT];
+  records<MT>(rec, h.it, img);
+  h.bias.load(h.it, rec, img, lane & 15, lane >> 4);
+  h.w.load(h.it.y, rec, 0, lane);
+}
+template <int BITS, int R, int MT, int UB>
+__device__ __forceinline__ void ahead_first(SnapAhead<BITS, R, MT, UB> &h, DescP nd, const char *img) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  h.it.y = layer_of(nd, 0); h.it.l = 0; h.it.s = (wave - waves) * MT;
+  h.any = next_item<MT>(h.it, nd, wave, waves);
+  if (h.any) ahead_load(h, img, lane);
+}
+
+// The inputs are in LDS, behind a barrier; `img`: the net's image, in memory (AHEAD: `h` comes from ahead_first, and whatever is
+// next, of the next layer too, is on its way while something is multiplied) or in LDS.  Ends with a barrier.
+template <int BITS, int R, int NT, int MT, int UB, bool AHEAD, class Out>
+__device__ __forceinline__ void net_tile(SnapAhead<BITS, R, MT, UB> &h, DescP nd, const SnapLds &m, const char *img, char *lds, Out out) {
+  using S = SnapShape<BITS, R, NT>;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, c = lane & 15, q = lane >> 4;
+  const int xrow = R == 16 ? c : (R == 4 ? c >> 2 : 0) + (BITS == 4 ? min(c & 3, 2) * S::T : 0);
+#pragma unroll 1
+  for (int l = 0; l < nd->L; ++l) {
+    const LayerOf y = layer_of(nd, l);
+    const int ldi = S::ld(y.in), ldo = S::ld(y.out);
+    const char *xin = lds + (l & 1 ? m.second : 0) + xrow * ldi + q * 16;
+    char *xout = lds + (l & 1 ? 0 : m.second);
+    const bool last = l == nd->L - 1;
+#pragma unroll 1
+    for (int s = wave * MT; s < y.strips; s += waves * MT) {
+      f32x4 acc[MT][NT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const char *rec[MT];
+      SnapBias<BITS, R, MT> bias;
+      if (AHEAD) {
+        records<MT>(rec, h.it, img);
+        h.bias.here();
+        bias = h.bias;
+      } else {
+        const Item it = {y, l, s};
+        records<MT>(rec, it, img);
+        bias.load(it, rec, img, c, q);
+      }
+#pragma unroll 1
+      for (int b = 0; b < y.steps; b += UB) {
+        SnapBlock<BITS, MT, UB> next;
+        if (AHEAD) {
+          h.w.here();
+          if (b + UB < y.steps) next.load(y, rec, b + UB, lane);
+        } else h.w.load(y, rec, b, lane);
+        if (b + UB <= y.steps) {
+#pragma unroll
+          for (int j = 0; j < UB; ++j) step_multiply<BITS, R, NT, MT>(h.w.w[j], h.w.sc[j / 4], 8 * (j & 3), acc, xin + (b + j) * 64, ldi);
+        } else {
+#pragma unroll
+          for (int j = 0; j < UB - 1; ++j)
+            if (j == 0 || b + j < y.steps) step_multiply<BITS, R, NT, MT>(h.w.w[j], h.w.sc[j / 4], 8 * (j & 3), acc, xin + (b + j) * 64, ldi);
+        }
+        if (AHEAD) h.w = next;
+      }
+      if (AHEAD && next_item<MT>(h.it, nd, wave, waves)) ahead_load(h, img, lane);
+      const bool odd = BITS == 4 && (y.strips & 1);            // the next layer's k-steps are 32 wide: zeros behind an odd last strip
+      if constexpr (R < 16) {
+        const int own = R > 1 ? 0 : BITS == 4 ? (c >> 2) & (MT - 1) : q & (MT - 1), at = BITS == 4 || R == 4 ? 4 * q + (c & 3) : c;
+#pragma unroll
+        for (int i = 0; i < (R == 1 ? 1 : MT); ++i) {
+          float v;
+          int strip = s + i;
+          if constexpr (R == 1 && BITS == 32) {                // the lanes (c, 0..3) hold parts of output c of every strip
+            float sum[MT];
+#pragma unroll
+            for (int k = 0; k < MT; ++k) {
+              const f32x4 p = acc[k][0];
+              sum[k] = (p[0] + p[1]) + (p[2] + p[3]);
+              sum[k] += __shfl_xor(sum[k], 16); sum[k] += __shfl_xor(sum[k], 32);
+            }
+            v = sum[0];
+#pragma unroll
+            for (int k = 1; k < MT; ++k) v = own == k ? sum[k] : v;
+            strip = s + own;
+          } else {
+            f32x4 p = acc[R == 1 ? 0 : i][0];
+            if constexpr (R == 1) {
+#pragma unroll
+              for (int k = 1; k < MT; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[j] = own == k ? acc[k][0][j] : p[j];
+              strip = s + own;
+            }
+            if constexpr (BITS == 4) {                         // the parts lie in the lanes of a quad: smallest first
+#pragma unroll
+              for (int j = 0; j < 4; ++j) p[j] = (quad_lane<2>(p[j]) + quad_lane<1>(p[j])) + quad_lane<0>(p[j]);
+            }
+            const int j = c & 3;
+            v = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
+          }
+          const int n = strip * 16 + at, t = R == 4 ? c >> 2 : 0;
+          v = act1(y.act, v + bias.v1[i]);
+          v = n < y.out ? v : 0.f;
+          const bool mine = strip < y.strips && (R == 4 || (BITS == 4 ? c < 4 * MT : q < MT));
+          if (mine) {
+            if (last) { if (n < y.out) out(t, n, v); }
+            else if constexpr (BITS == 4) {
+              float p[3];
+              split3(v, p);
+#pragma unroll
+              for (int k = 0; k < 3; ++k) {
+                char *o = xout + (k * S::T + t) * ldo + n * 2;
+                *(unsigned short *)o = bf_top(p[k]);
+                if (odd && strip == y.strips - 1) *(unsigned short *)(o + 32) = 0;
+              }
+            } else *(float *)(xout + t * ldo + n * 4) = v;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          if (s + i < y.strips) {
+            const int n0 = (s + i) * 16 + 4 * q;
+            const bool end = s + i == y.strips - 1;
+#pragma unroll
+            for (int tt = 0; tt < NT; ++tt) {
+              const int t = 16 * tt + c;
+              f32x4 a = act4(y.act, acc[i][tt] + bias.v4[i]);
+              if (end) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) a[j] = n0 + j < y.out ? a[j] : 0.f;
+              }
+              if (last) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) if (n0 + j < y.out) out(t, n0 + j, a[j]);
+              } else if constexpr (BITS == 4) {
+                float p[4][3];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) split3(a[j], p[j]);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) {
+                  char *o = xout + (k * S::T + t) * ldo + n0 * 2;
+                  *(u32x2 *)o = u32x2{two_tops(p[0][k], p[1][k]), two_tops(p[2][k], p[3][k])};
+                  if (odd && end) *(u32x2 *)(o + 32) = u32x2{0u, 0u};
+                }
+              } else *(f32x4 *)(xout + t * ldo + n0 * 4) = a;
+            }
+          }
+      }
+    }
+    lds_barrier();
+  }
+}
+
+// A net's image from memory to LDS, without a register in between: everything is asked for at once.  The caller waits.
+__device__ __forceinline__ void image_in(const char *img, char *lds, unsigned bytes) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (unsigned i = wave * 1024; i < bytes; i += waves * 1024)
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(img + i + lane * 16),
+                                     (__attribute__((address_space(3))) void *)(lds + i), 16, 0, 0);
+}
+__device__ __forceinline__ void image_here() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // ------------------------------------------------------------------------------------------------------------------------
 // Every agent's net on its rows
 // ------------------------------------------------------------------------------------------------------------------------
-template <int BITS, int NT, bool PACK>
-__global__ void __launch_bounds__(256)
-snap_forward_kernel(const SnapDesc nd, const SnapLds m, const SnapForward p) {
+template <int BITS, int R, int NT, int MT, int UB, bool STAGE>
+__global__ void __launch_bounds__(512)
+snap_forward_kernel(const SnapDesc nd_, const SnapLds m, const SnapForward p) {
   extern __shared__ __align__(16) char lds[];
-  using S = SnapShape<BITS, NT, PACK>;
+  using S = SnapShape<BITS, R, NT>;
+  const DescP nd = SNAP_DESC(nd_);
   const int g = blockIdx.x;
   if (p.mask && !p.mask[g]) return;
-  const char *img = p.img + (size_t)g * nd.stride;
+  const char *img = p.img + (size_t)g * nd->stride;
+  if (STAGE) { image_in(img, lds + m.image, nd->stride); img = lds + m.image; }
   const int from = blockIdx.y * p.per, to = min(p.n, from + p.per);
+#pragma unroll 1
   for (int t0 = from; t0 < to; t0 += S::T) {
+    SnapAhead<BITS, R, MT, UB> h;
+    if (!STAGE) ahead_first(h, nd, img);
     const float *x = p.x + g * p.x_agent + t0 * p.x_row;
-    tile_in<BITS, NT, PACK>(nd.in[0], lds, [&](int t) { return t0 + t < to ? x + t * p.x_row : (const float *)nullptr; });
-    __syncthreads();
+    tile_in<BITS, R, NT>(nd->lay[0].in, lds, [&](int t) { return t0 + t < to ? x + t * p.x_row : (const float *)nullptr; });
+    if (STAGE) image_here();
+    lds_barrier();
     float *o = p.out + g * p.out_agent + t0 * p.out_row;
-    net_tile<BITS, NT, PACK>(nd, m, img, lds, [&](int t, int n, float v) { if (t0 + t < to) o[t * p.out_row + n] = v; });
+    net_tile<BITS, R, NT, MT, UB, !STAGE>(h, nd, m, img, lds, [&](int t, int n, float v) { if (t0 + t < to) o[t * p.out_row + n] = v; });
   }
 }
 
@@ -300,47 +506,107 @@ __device__ __forceinline__ double key_logit(unsigned long long k) {
 }
 __device__ __forceinline__ bool key_before(unsigned long long ka, int ia, unsigned long long kb, int ib) { return ka > kb || (ka == kb && ia < ib); }
 
+// The best of 16 lanes' (key, index), in all of them.  quad_perm and the mirrors reach every lane of a row of 16.
+template <int CTRL>
+__device__ __forceinline__ void best_dpp(unsigned long long &k, int &i) {
+  const int hi = (int)(k >> 32), lo = (int)k;
+  const unsigned oh = (unsigned)__builtin_amdgcn_update_dpp(0, hi, CTRL, 0xf, 0xf, true), ol = (unsigned)__builtin_amdgcn_update_dpp(0, lo, CTRL, 0xf, 0xf, true);
+  const int oi = __builtin_amdgcn_update_dpp(0, i, CTRL, 0xf, 0xf, true);
+  const unsigned long long ok = (unsigned long long)oh << 32 | ol;
+  if (key_before(ok, oi, k, i)) { k = ok; i = oi; }
+}
+__device__ __forceinline__ void best_of_16(unsigned long long &k, int &i) {
+  best_dpp<0xB1>(k, i); best_dpp<0x4E>(k, i); best_dpp<0x141>(k, i); best_dpp<0x140>(k, i);
+}
+#define IDX_NONE 0x7fffffff
+__device__ __forceinline__ int lane_of_16(int v, int j) { return __shfl(v, j, 16); }
+
+// A row's picks from sorted lists of k: lane u of 16 looks at list u (lists <= 16), lane j keeps the j-th pick: its index (or
+// IDX_NONE) and, after the softmax, its probability
+template <class Key, class Idx>
+__device__ __forceinline__ void merge_16(int u, int lists, int k, Key key, Idx idx, int &mi, float &mp) {
+  int head = 0;
+  unsigned long long mk = KEY_NONE, nk = KEY_NONE;
+  int ni = IDX_NONE;
+  mi = IDX_NONE;
+  if (u < lists) { nk = key(0); ni = idx(0); }
+  for (int j = 0; j < k; ++j) {
+    unsigned long long bk = nk;
+    int bi = ni;
+    best_of_16(bk, bi);
+    if (bi != IDX_NONE && ni == bi) {
+      ++head;
+      const bool more = head < k;
+      nk = more ? key(head) : KEY_NONE; ni = more ? idx(head) : IDX_NONE;
+    }
+    if (u == j) { mk = bk; mi = bi; }
+  }
+  const double l = key_logit(mk), top = __shfl(l, 0, 16);
+  const float ex = mi != IDX_NONE ? expf((float)(l - top)) : 0.f;
+  float sum = 0.f;
+  for (int j = 0; j < k; ++j) sum += __shfl(ex, j, 16);
+  mp = mi != IDX_NONE ? ex / sum : 0.f;
+}
+
+// grid (rows / 16, chunks): the rows' best among the agents [chunk * G / chunks, ..); with one chunk the picks themselves
 template <int KM>
 __global__ void __launch_bounds__(1024)
 snap_router_kernel(const SnapMixture p, int S, int A, int ld) {
   extern __shared__ __align__(16) char lds[];
   float *xs = (float *)lds;                                // [16][ld]
-  const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   unsigned long long *ck = (unsigned long long *)(lds + 16 * ld * 4);       // [16][waves][KM]
   int *ci = (int *)(ck + 16 * waves * KM);
   const int t0 = blockIdx.x * 16;
+  const int strips = (p.G + 15) >> 4, each = (strips + p.chunks - 1) / p.chunks, s_from = blockIdx.y * each, s_to = min(strips, s_from + each);
   const int Sp = (S + 15) & ~15;
-  for (int i = threadIdx.x; i < 16 * Sp; i += blockDim.x) {
-    const int t = i / Sp, k = i - t * Sp;
-    xs[t * ld + k] = t0 + t < p.n && k < S ? p.x[(t0 + t) * p.x_row + k] : 0.f;
-  }
-  __syncthreads();
+  for (int t = threadIdx.x >> 5; t < 16; t += blockDim.x >> 5)
+    for (int k = threadIdx.x & 31; k < Sp; k += 32) xs[t * ld + k] = t0 + t < p.n && k < S ? p.x[(t0 + t) * p.x_row + k] : 0.f;
   unsigned long long K[KM];
   int I[KM];
 #pragma unroll
-  for (int j = 0; j < KM; ++j) { K[j] = KEY_NONE; I[j] = 0x7fffffff; }
+  for (int j = 0; j < KM; ++j) { K[j] = KEY_NONE; I[j] = IDX_NONE; }
   const int row = min(t0 + c, p.n - 1);
   const uint8_t *al = p.allowed ? p.allowed + row * p.a_row : nullptr;
-  for (int s = wave; s * 16 < p.G; s += waves) {
+  bool first = true;
+  for (int s = s_from + wave; s < s_to; s += waves) {
     const float *w = p.rw + (int64_t)min(s * 16 + c, p.G - 1) * p.r_row;
+    float bias[4];
+    bool ok[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int e = min(s * 16 + 4 * j + q, p.G - 1);
+      bias[j] = p.rb ? p.rb[e] : 0.f;
+      ok[j] = (!al || al[e]) && s * 16 + 4 * j + q < p.G;
+    }
     f64x4 acc = {0., 0., 0., 0.};
-    for (int k = 0; k < S; k += 16) {
-      const int at = k + 4 * q;
-      float a[4];
-      if (at + 3 < S) { const f32x4u v = *(const f32x4u *)(w + at); a[0] = v[0]; a[1] = v[1]; a[2] = v[2]; a[3] = v[3]; }
-      else {
+    constexpr int U = KM > 4 ? 2 : 4;                       // 16 inputs each, asked for together
+    for (int k0 = 0; k0 < S; k0 += 16 * U) {
+      float a[U][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] = at + j < S ? w[at + j] : 0.f;
+      for (int u = 0; u < U; ++u) {
+        const int at = k0 + 16 * u + 4 * q;
+        if (k0 + 16 * u + 16 <= S) {
+          const f32x4u v = *(const f32x4u *)(w + at);
+          a[u][0] = v[0]; a[u][1] = v[1]; a[u][2] = v[2]; a[u][3] = v[3];
+        } else if (k0 + 16 * u < S) {                       // the row's end: no lane reads beyond it
+#pragma unroll
+          for (int j = 0; j < 4; ++j) { const float v = w[min(at + j, S - 1)]; a[u][j] = at + j < S ? v : 0.f; }
+        }
       }
-      const f32x4 x = *(const f32x4 *)(xs + c * ld + at);
+      if (first) { __syncthreads(); first = false; }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)a[j], (double)x[j], acc, 0, 0, 0);
+      for (int u = 0; u < U; ++u)
+        if (k0 + 16 * u < S) {
+          const f32x4 x = *(const f32x4 *)(xs + c * ld + k0 + 16 * u + 4 * q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)a[u][j], (double)x[j], acc, 0, 0, 0);
+        }
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       int e = s * 16 + 4 * j + q;
-      unsigned long long key = KEY_NONE;
-      if (e < p.G && (!al || al[e])) key = logit_key(acc[j] + (p.rb ? (double)p.rb[e] : 0.));
+      unsigned long long key = ok[j] ? logit_key(acc[j] + (double)bias[j]) : KEY_NONE;
       if (key > K[KM - 1]) {
 #pragma unroll
         for (int i = 0; i < KM; ++i) {
@@ -352,6 +618,7 @@ snap_router_kernel(const SnapMixture p, int S, int A, int ld) {
       }
     }
   }
+  if (first) __syncthreads();
   // the four lanes of a row
   for (int j = 0; j < p.k; ++j) {
     unsigned long long bk = K[0];
@@ -365,94 +632,161 @@ snap_router_kernel(const SnapMixture p, int S, int A, int ld) {
     if (I[0] == bi) {
 #pragma unroll
       for (int i = 0; i + 1 < KM; ++i) { K[i] = K[i + 1]; I[i] = I[i + 1]; }
-      K[KM - 1] = KEY_NONE; I[KM - 1] = 0x7fffffff;
+      K[KM - 1] = KEY_NONE; I[KM - 1] = IDX_NONE;
     }
     if (q == 0) { ck[(c * waves + wave) * KM + j] = bk; ci[(c * waves + wave) * KM + j] = bi; }
   }
   __syncthreads();
-  // the waves: 16 lanes a row, lane u holds wave u's list; lane j keeps the j-th pick
+  // the waves: 16 lanes a row
   const int u = threadIdx.x & 15;
   for (int t = threadIdx.x >> 4; t < 16; t += blockDim.x >> 4) {
     const int tok = t0 + t;
-    const bool live = tok < p.n;
-    int head = 0, mi = 0x7fffffff;
-    unsigned long long mk = KEY_NONE;
-    for (int j = 0; j < p.k; ++j) {
-      unsigned long long bk = KEY_NONE;
-      int bi = 0x7fffffff;
-      if (u < waves && head < p.k) { bk = ck[(t * waves + u) * KM + head]; bi = ci[(t * waves + u) * KM + head]; }
-      const int own = bi;
-#pragma unroll
-      for (int d = 1; d <= 8; d *= 2) {
-        const unsigned long long ok = __shfl_xor(bk, d);
-        const int oi = __shfl_xor(bi, d);
-        if (key_before(ok, oi, bk, bi)) { bk = ok; bi = oi; }
+    const unsigned long long *lk = ck + (t * waves + (u < waves ? u : 0)) * KM;
+    const int *li = ci + (t * waves + (u < waves ? u : 0)) * KM;
+    if (p.chunks > 1) {                                    // the chunk's list, sorted
+      int head = 0;
+      for (int j = 0; j < p.k; ++j) {
+        unsigned long long bk = KEY_NONE;
+        int bi = IDX_NONE;
+        if (u < waves && head < p.k) { bk = lk[head]; bi = li[head]; }
+        const int own = bi;
+        best_of_16(bk, bi);
+        if (own == bi && bi != IDX_NONE) ++head;
+        if (tok < p.n && u == j) {
+          p.ckey[((int64_t)tok * p.chunks + blockIdx.y) * p.k + j] = bk;
+          p.cidx[((int64_t)tok * p.chunks + blockIdx.y) * p.k + j] = bi;
+        }
       }
-      if (own == bi && bi != 0x7fffffff) ++head;
-      if (u == j) { mk = bk; mi = bi; }
+      if (tok < p.n && u == 0 && blockIdx.y == 0) p.count[tok] = 0;
+      continue;
     }
-    const bool have = mi != 0x7fffffff;
-    const double l = key_logit(mk), top = __shfl(l, 0, 16);
-    const float ex = have ? expf((float)(l - top)) : 0.f;
-    float sum = 0.f;
-    for (int j = 0; j < p.k; ++j) sum += __shfl(ex, j, 16);
+    int mi;
+    float mp;
+    merge_16(u, waves, p.k, [&](int h) { return lk[h]; }, [&](int h) { return li[h]; }, mi, mp);
+    const bool have = mi != IDX_NONE, live = tok < p.n;
     if (live && u < p.k) {
       p.idx[(int64_t)tok * p.k + u] = have ? mi : -1;
-      p.prob[(int64_t)tok * p.k + u] = have ? ex / sum : 0.f;
+      p.prob[(int64_t)tok * p.k + u] = mp;
       if (!have) for (int a = 0; a < A; ++a) p.y[((int64_t)tok * p.k + u) * A + a] = 0.f;
     }
-    const int first = __shfl(mi, 0, 16);
-    if (live && first == 0x7fffffff) for (int a = u; a < A; a += 16) p.out[tok * p.out_row + a] = 0.f;
+    if (live && lane_of_16(mi, 0) == IDX_NONE) for (int a = u; a < A; a += 16) p.out[tok * p.out_row + a] = 0.f;
     if (live && u == 0) p.count[tok] = 0;
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
-// The picked nets.  A workgroup answers, for one net, the places (row, j) of a piece of idx that picked it, T at a time, and
-// whoever answers a row's last place sums the row up, in the order of its places whatever the order they were answered in.
-// Few places: one workgroup per place, and the first place of a net takes the others along; many: one per (net, piece).
+// The picked nets, few places: a workgroup for each.  It makes the row's picks out of the router's lists (or reads them), answers
+// its place, and whoever answers a row's last place sums the row up, in the order of its places whatever the order they were
+// answered in.  The answers are stored past the XCD's own cache (agent scope); once they have arrived the counter may tell of
+// them.  Nothing else passes between workgroups, so no cache has to be written back or forgotten, and nobody waits.
+// ------------------------------------------------------------------------------------------------------------------------
+template <int BITS, int MT, int UB, bool STAGE>
+__global__ void __launch_bounds__(512)
+snap_place_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ int picks[SNAP_MAXK], last;
+  __shared__ float probs[SNAP_MAXK];
+  const DescP nd = SNAP_DESC(nd_);
+  const int tid = threadIdx.x, A = nd->A, row = blockIdx.x / p.k, place = blockIdx.x - row * p.k;
+  if (p.chunks > 1) {
+    if (tid < 16) {
+      int mi;
+      float mp;
+      const int64_t at = ((int64_t)row * p.chunks + (tid < p.chunks ? tid : 0)) * p.k;
+      merge_16(tid, p.chunks, p.k, [&](int h) { return p.ckey[at + h]; }, [&](int h) { return p.cidx[at + h]; }, mi, mp);
+      if (tid < p.k) { picks[tid] = mi == IDX_NONE ? -1 : mi; probs[tid] = mp; }
+    }
+  } else if (tid < p.k) { picks[tid] = p.idx[row * p.k + tid]; probs[tid] = p.prob[row * p.k + tid]; }
+  __syncthreads();
+  const int e = __builtin_amdgcn_readfirstlane(picks[place]);
+  float *y = p.y + (int64_t)blockIdx.x * A;
+  if (p.chunks > 1) {
+    if (tid == 0) { p.idx[blockIdx.x] = e; p.prob[blockIdx.x] = probs[place]; }
+    if (e < 0) {
+      for (int a = tid; a < A; a += blockDim.x) y[a] = 0.f;
+      if (picks[0] < 0 && place == 0) for (int a = tid; a < A; a += blockDim.x) p.out[row * p.out_row + a] = 0.f;
+    }
+  }
+  if (e < 0) return;
+  const char *img = p.img + (size_t)e * nd->stride;
+  SnapAhead<BITS, 1, MT, UB> h;
+  if (STAGE) { image_in(img, lds + m.image, nd->stride); img = lds + m.image; }
+  else ahead_first(h, nd, img);
+  const float *x = p.x + row * p.x_row;
+  tile_in<BITS, 1, 1>(nd->lay[0].in, lds, [&](int) { return x; });
+  if (STAGE) image_here();
+  lds_barrier();
+  net_tile<BITS, 1, 1, MT, UB, !STAGE>(h, nd, m, img, lds, [&](int, int n, float v) { __hip_atomic_store(y + n, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    int want = 0;
+    for (int j = 0; j < p.k; ++j) want += picks[j] >= 0;
+    last = __hip_atomic_fetch_add(p.count + row, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == want - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  for (int a = tid; a < A; a += blockDim.x) {
+    float sum = 0.f;
+    for (int j = 0; j < p.k; ++j)
+      if (picks[j] >= 0) sum = fmaf(probs[j], __hip_atomic_load(p.y + ((int64_t)row * p.k + j) * A + a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), sum);
+    p.out[row * p.out_row + a] = sum;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------
+// The picked nets, many places: a workgroup answers, for one net, the places of a piece of idx that picked it, T at a time; the
+// rows are summed up as above.
 // ------------------------------------------------------------------------------------------------------------------------
 #define SNAP_LIST 1024
-template <int BITS, int NT, bool PACK>
-__global__ void __launch_bounds__(256)
-snap_experts_kernel(const SnapDesc nd, const SnapLds m, const SnapMixture p, int by_place, int piece) {
+template <int BITS, int R, int NT, int MT, int UB, bool STAGE>
+__global__ void __launch_bounds__(512)
+snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p, int piece) {
   extern __shared__ __align__(16) char lds[];
-  using S = SnapShape<BITS, NT, PACK>;
-  __shared__ int list[SNAP_LIST + 256], cnt, done[16 * NT > 5 ? 16 * NT : 5];
-  const int tid = threadIdx.x, A = nd.A, total = p.n * p.k;
-  int e, from, to;
-  if (by_place) {
-    from = blockIdx.x; to = total;
-    e = p.idx[from];
-    if (e < 0) return;
-    int before = 0;
-    for (int i = tid; i < from; i += 256) before |= p.idx[i] == e;
-    if (__syncthreads_or(before)) return;
-  } else {
-    e = blockIdx.x;
-    from = blockIdx.y * piece; to = min(total, from + piece);
-  }
-  const char *img = p.img + (size_t)e * nd.stride;
+  using S = SnapShape<BITS, R, NT>;
+  __shared__ int list[SNAP_LIST + 2048], cnt, done[S::T];
+  const DescP nd = SNAP_DESC(nd_);
+  const int tid = threadIdx.x, A = nd->A, total = p.n * p.k, threads = blockDim.x, e = blockIdx.x;
+  int from = blockIdx.y * piece;
+  const int to = min(total, from + piece);
+  const char *img = p.img + (size_t)e * nd->stride;
+  bool staged = false;
   while (from < to) {
+    __syncthreads();
     if (tid == 0) cnt = 0;
     __syncthreads();
-    for (;;) {                                             // from and cnt are the same in all threads
-      const int i = from + tid;
-      if (i < to && p.idx[i] == e) list[atomicAdd(&cnt, 1)] = i;
-      from += 256;
+    for (;;) {                                             // 4 places a thread and round
+      int v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { const int i = from + j * threads + tid; v[j] = i < to ? p.idx[i] : -1; }
+      int mine = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mine += v[j] == e;
+      if (mine) {
+        int at = atomicAdd(&cnt, mine);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (v[j] == e) list[at++] = from + j * threads + tid;
+      }
+      from += 4 * threads;
+      if (from >= to) break;
       __syncthreads();
       const int have = cnt;
       __syncthreads();
-      if (from >= to || have > SNAP_LIST) break;
+      if (have > SNAP_LIST) break;
     }
+    __syncthreads();
     const int have = cnt;
+    if (STAGE && have && !staged) { image_in(img, lds + m.image, nd->stride); img = lds + m.image; staged = true; }
     for (int i0 = 0; i0 < have; i0 += S::T) {
-      tile_in<BITS, NT, PACK>(nd.in[0], lds, [&](int t) { return i0 + t < have ? p.x + (int64_t)(list[i0 + t] / p.k) * p.x_row : (const float *)nullptr; });
-      __syncthreads();
-      net_tile<BITS, NT, PACK>(nd, m, img, lds, [&](int t, int n, float v) {
+      SnapAhead<BITS, R, MT, UB> h;
+      if (!STAGE) ahead_first(h, nd, img);
+      tile_in<BITS, R, NT>(nd->lay[0].in, lds, [&](int t) { return i0 + t < have ? p.x + (int64_t)(list[i0 + t] / p.k) * p.x_row : (const float *)nullptr; });
+      if (STAGE) image_here();
+      lds_barrier();
+      net_tile<BITS, R, NT, MT, UB, !STAGE>(h, nd, m, img, lds, [&](int t, int n, float v) {
         if (i0 + t < have) __hip_atomic_store(p.y + (int64_t)list[i0 + t] * A + n, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       });
-      __threadfence();
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       if (tid < S::T) {
         int row = -1;
@@ -460,13 +794,12 @@ snap_experts_kernel(const SnapDesc nd, const SnapLds m, const SnapMixture p, int
           const int r = list[i0 + tid] / p.k;
           int want = 0;
           for (int j = 0; j < p.k; ++j) want += p.idx[r * p.k + j] >= 0;
-          if (__hip_atomic_fetch_add(p.count + r, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == want - 1) row = r;
+          if (__hip_atomic_fetch_add(p.count + r, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == want - 1) row = r;
         }
         done[tid] = row;
       }
       __syncthreads();
-      __threadfence();
-      for (int i = tid; i < S::T * A; i += 256) {
+      for (int i = tid; i < S::T * A; i += threads) {
         const int t = i / A, a = i - t * A, r = done[t];
         if (r < 0) continue;
         float sum = 0.f;
@@ -573,76 +906,115 @@ snap_grad_kernel(const SnapGrad p) {
 // ------------------------------------------------------------------------------------------------------------------------
 // launches
 // ------------------------------------------------------------------------------------------------------------------------
-template <int BITS, int NT, bool PACK>
+static int most_strips(const SnapDesc &nd) {
+  int most = 0;
+  for (int l = 0; l < nd.L; ++l) most = nd.lay[l].strips > most ? nd.lay[l].strips : most;
+  return most;
+}
+#define SNAP_STAGE (64 * 1024)      // images up to here are staged: two workgroups and more of them fit a CU
+template <int BITS, int R, int NT, int MT, int UB, bool STAGE>
 static hipError_t forward_run(const SnapDesc &nd, SnapForward p, hipStream_t st) {
   SnapLds m;
-  const int lds = SnapShape<BITS, NT, PACK>::bytes(nd, m), T = SnapShape<BITS, NT, PACK>::T;
+  const int lds = SnapShape<BITS, R, NT>::bytes(nd, m) + (STAGE ? nd.stride : 0), T = R * NT;
   static LdsConfig cfg;
-  hipError_t e = ddrl_set_lds(snap_forward_kernel<BITS, NT, PACK>, lds, cfg);
+  const auto kernel = snap_forward_kernel<BITS, R, NT, MT, UB, STAGE>;
+  hipError_t e = ddrl_set_lds(kernel, lds, cfg);
   if (e != hipSuccess) return e;
   const int tiles = (p.n + T - 1) / T;
   int chunks = p.G >= 1024 ? 1 : (1024 + p.G - 1) / p.G;
   if (chunks > tiles) chunks = tiles;
   const int per = (tiles + chunks - 1) / chunks;
   p.per = per * T;
-  hipLaunchKernelGGL((snap_forward_kernel<BITS, NT, PACK>), dim3(p.G, (tiles + per - 1) / per), dim3(256), lds, st, nd, m, p);
+  int waves = (most_strips(nd) + MT - 1) / MT;
+  waves = waves > 8 ? 8 : waves;
+  hipLaunchKernelGGL(kernel, dim3(p.G, (tiles + per - 1) / per), dim3(waves * 64), lds, st, nd, m, p);
   return hipGetLastError();
 }
-template <int BITS, int NT, bool PACK>
-static bool fits(const SnapDesc &nd, int more) { SnapLds m; return SnapShape<BITS, NT, PACK>::bytes(nd, m) + more <= SNAP_LDS; }
+template <int BITS, int R, int NT>
+static bool fits(const SnapDesc &nd, int more) { SnapLds m; return SnapShape<BITS, R, NT>::bytes(nd, m) + more <= SNAP_LDS; }
 
 extern "C" hipError_t snap_forward_launch(const SnapDesc *nd, const SnapForward *p, hipStream_t st) {
+  const int img = nd->stride;
+  const bool stage = img <= SNAP_STAGE;
   if (nd->bits == 4) {
-    if (p->n > 16 && fits<4, 2, false>(*nd, 0)) return forward_run<4, 2, false>(*nd, *p, st);
-    if (p->n > 5 && fits<4, 1, false>(*nd, 0)) return forward_run<4, 1, false>(*nd, *p, st);
-    return forward_run<4, 1, true>(*nd, *p, st);
+    if (p->n > 16 && stage && fits<4, 16, 2>(*nd, img)) return forward_run<4, 16, 2, 2, 4, true>(*nd, *p, st);
+    if (p->n > 4 && stage && fits<4, 16, 1>(*nd, img)) return forward_run<4, 16, 1, 2, 4, true>(*nd, *p, st);
+    if (p->n > 4 && fits<4, 16, 1>(*nd, 0)) return forward_run<4, 16, 1, 4, 4, false>(*nd, *p, st);
+    if (p->n > 1 && stage && fits<4, 4, 1>(*nd, img)) return forward_run<4, 4, 1, 2, 4, true>(*nd, *p, st);
+    if (p->n > 1) return forward_run<4, 4, 1, 2, 4, false>(*nd, *p, st);
+    if (stage && fits<4, 1, 1>(*nd, img)) return forward_run<4, 1, 1, 2, 4, true>(*nd, *p, st);
+    return forward_run<4, 1, 1, 2, 4, false>(*nd, *p, st);
   }
-  if (p->n > 16 && fits<32, 2, false>(*nd, 0)) return forward_run<32, 2, false>(*nd, *p, st);
-  return forward_run<32, 1, false>(*nd, *p, st);
+  if (p->n > 16 && fits<32, 16, 2>(*nd, 0)) return forward_run<32, 16, 2, 2, 4, false>(*nd, *p, st);
+  if (p->n > 1 && stage && fits<32, 16, 1>(*nd, img)) return forward_run<32, 16, 1, 2, 4, true>(*nd, *p, st);
+  if (p->n > 1) return forward_run<32, 16, 1, 2, 4, false>(*nd, *p, st);
+  if (stage && fits<32, 1, 1>(*nd, img)) return forward_run<32, 1, 1, 2, 4, true>(*nd, *p, st);
+  return forward_run<32, 1, 1, 2, 4, false>(*nd, *p, st);
 }
 
 template <int KM>
 static hipError_t router_run(const SnapMixture &p, int S, int A, hipStream_t st) {
   const int ld = ddrl_roundup(S, 64) + 4;
+  const int strips = ((p.G + 15) / 16 + p.chunks - 1) / p.chunks;
   int waves = 4;
-  while (waves < 16 && waves * 16 < p.G) waves *= 2;
+  while (waves < 16 && waves < strips) waves *= 2;
   const size_t lds = (size_t)16 * ld * 4 + (size_t)16 * waves * KM * 12;
   static LdsConfig cfg;
   hipError_t e = ddrl_set_lds(snap_router_kernel<KM>, lds, cfg);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(snap_router_kernel<KM>, dim3((p.n + 15) / 16), dim3(waves * 64), lds, st, p, S, A, ld);
+  hipLaunchKernelGGL(snap_router_kernel<KM>, dim3((p.n + 15) / 16, p.chunks), dim3(waves * 64), lds, st, p, S, A, ld);
   return hipGetLastError();
 }
-template <int BITS, int NT, bool PACK>
+static int waves_for(const SnapDesc &nd, int mt) {
+  const int waves = (most_strips(nd) + mt - 1) / mt;
+  return waves > 8 ? 8 : waves;
+}
+template <int BITS, int MT, int UB, bool STAGE>
+static hipError_t place_run(const SnapDesc &nd, const SnapMixture &p, hipStream_t st) {
+  SnapLds m;
+  const int lds = SnapShape<BITS, 1, 1>::bytes(nd, m) + (STAGE ? nd.stride : 0);
+  static LdsConfig cfg;
+  const auto kernel = snap_place_kernel<BITS, MT, UB, STAGE>;
+  hipError_t e = ddrl_set_lds(kernel, lds, cfg);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(kernel, dim3(p.n * p.k), dim3(waves_for(nd, MT) * 64), lds, st, nd, m, p);
+  return hipGetLastError();
+}
+template <int BITS, int R, int NT, int MT, int UB, bool STAGE>
 static hipError_t experts_run(const SnapDesc &nd, const SnapMixture &p, hipStream_t st) {
   SnapLds m;
-  const int lds = SnapShape<BITS, NT, PACK>::bytes(nd, m);
+  const int lds = SnapShape<BITS, R, NT>::bytes(nd, m) + (STAGE ? nd.stride : 0);
   static LdsConfig cfg;
-  hipError_t e = ddrl_set_lds(snap_experts_kernel<BITS, NT, PACK>, lds, cfg);
+  const auto kernel = snap_experts_kernel<BITS, R, NT, MT, UB, STAGE>;
+  hipError_t e = ddrl_set_lds(kernel, lds, cfg);
   if (e != hipSuccess) return e;
-  const int total = p.n * p.k;
-  if (total <= 1024) {
-    hipLaunchKernelGGL((snap_experts_kernel<BITS, NT, PACK>), dim3(total), dim3(256), lds, st, nd, m, p, 1, 0);
-  } else {
-    int pieces = (1024 + p.G - 1) / p.G;
-    int piece = ddrl_roundup((total + pieces - 1) / pieces, 256);
-    hipLaunchKernelGGL((snap_experts_kernel<BITS, NT, PACK>), dim3(p.G, (total + piece - 1) / piece), dim3(256), lds, st, nd, m, p, 0, piece);
-  }
+  int waves = waves_for(nd, MT);
+  waves = waves < 4 ? 4 : waves;
+  const int total = p.n * p.k, pieces = (1024 + p.G - 1) / p.G;
+  const int piece = ddrl_roundup((total + pieces - 1) / pieces, 1024);
+  hipLaunchKernelGGL(kernel, dim3(p.G, (total + piece - 1) / piece), dim3(waves * 64), lds, st, nd, m, p, piece);
   return hipGetLastError();
 }
 
-#define SNAP_STATIC_LDS 8192         // snap_experts_kernel's list and flags
+#define SNAP_STATIC_LDS 13312        // snap_experts_kernel's list and flags
 extern "C" hipError_t snap_mixture_launch(const SnapDesc *nd, const SnapMixture *p, hipStream_t st) {
-  const int S = nd->d[0], A = nd->d[nd->L];
+  const int S = nd->lay[0].in, A = nd->A;
   hipError_t e = p->k == 1 ? router_run<1>(*p, S, A, st) : p->k == 2 ? router_run<2>(*p, S, A, st) : p->k <= 4 ? router_run<4>(*p, S, A, st)
                                                                                                               : router_run<8>(*p, S, A, st);
   if (e != hipSuccess) return e;
-  const int total = p->n * p->k;
-  if (nd->bits == 4) {
-    if (total > 5 * p->G && fits<4, 1, false>(*nd, SNAP_STATIC_LDS)) return experts_run<4, 1, false>(*nd, *p, st);
-    return experts_run<4, 1, true>(*nd, *p, st);
+  const int total = p->n * p->k, img = nd->stride;
+  const bool stage = img <= SNAP_STAGE;
+  if (total <= SNAP_FEW) {
+    if (nd->bits == 4) return stage ? place_run<4, 2, 4, true>(*nd, *p, st) : place_run<4, 2, 4, false>(*nd, *p, st);
+    return stage ? place_run<32, 2, 4, true>(*nd, *p, st) : place_run<32, 2, 4, false>(*nd, *p, st);
   }
-  return experts_run<32, 1, false>(*nd, *p, st);
+  if (nd->bits == 4) {
+    if (stage && fits<4, 16, 1>(*nd, SNAP_STATIC_LDS + img)) return experts_run<4, 16, 1, 2, 4, true>(*nd, *p, st);
+    if (fits<4, 16, 1>(*nd, SNAP_STATIC_LDS)) return experts_run<4, 16, 1, 4, 4, false>(*nd, *p, st);
+    return experts_run<4, 4, 1, 2, 4, false>(*nd, *p, st);
+  }
+  if (stage && fits<32, 16, 1>(*nd, SNAP_STATIC_LDS + img)) return experts_run<32, 16, 1, 2, 4, true>(*nd, *p, st);
+  return experts_run<32, 16, 1, 2, 4, false>(*nd, *p, st);
 }
 
 extern "C" hipError_t snap_grad_launch(const SnapGrad *p, hipStream_t st) {

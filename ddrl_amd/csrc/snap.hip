@@ -29,7 +29,7 @@ struct DevBuf {                        // temporary device memory of a host-buff
 };
 bool off4(const void *p) { return ((uintptr_t)p & 3) != 0; }
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
-struct MixSpace { size_t count, idx, prob, y, all; };
+struct MixSpace { size_t count, idx, prob, y, ckey, cidx, all; int chunks; };
 MixSpace mix_space(const ddrl_snap *s, int n, int k) {
   MixSpace w;
   const size_t places = (size_t)n * k;
@@ -37,7 +37,11 @@ MixSpace mix_space(const ddrl_snap *s, int n, int k) {
   w.idx = up16((size_t)n * 4);
   w.prob = w.idx + up16(places * 4);
   w.y = w.prob + up16(places * 4);
-  w.all = w.y + up16(places * s->nd.d[s->nd.L] * 4);
+  w.ckey = w.y + up16(places * s->nd.A * 4);
+  w.chunks = snap_chunks(s->G, n, k);
+  const size_t lists = w.chunks > 1 ? places * w.chunks : 0;
+  w.cidx = w.ckey + up16(lists * 8);
+  w.all = w.cidx + up16(lists * 4);
   return w;
 }
 int check_mix_shape(const ddrl_snap *s, int n, int k) {
@@ -118,8 +122,8 @@ extern "C" int ddrl_snap_create_from(ddrl_pop_t *h, int net, int bits, ddrl_snap
 extern "C" int ddrl_snap_shape(ddrl_snap_t *s, int *n_agents, int *in_dim, int *out_dim, int *bits, int *n_params) {
   if (!s) return ddrl_fail(DDRL_EINVAL, "NULL handle");
   if (n_agents) *n_agents = s->G;
-  if (in_dim) *in_dim = s->nd.d[0];
-  if (out_dim) *out_dim = s->nd.d[s->nd.L];
+  if (in_dim) *in_dim = s->nd.lay[0].in;
+  if (out_dim) *out_dim = s->nd.A;
   if (bits) *bits = s->nd.bits;
   if (n_params) *n_params = s->nd.np;
   return DDRL_OK;
@@ -138,8 +142,9 @@ extern "C" int ddrl_snap_load(ddrl_snap_t *s, ddrl_pop_t *h, int net, void *stre
   const NetDesc &n = train_net(h, net)->nd;
   if (n.bn_any()) return ddrl_fail(DDRL_EINVAL, "net %d has BatchNorm towers: a snapshot holds InnerProducts only", net);
   if (h->gates_on) return ddrl_fail(DDRL_ESTATE, "developmental gates are in force: a snapshot holds the nets alone");
-  bool same = h->G == s->G && n.L() == s->nd.L && n.hidden_act() == s->nd.hact && n.out_act() == s->nd.oact && h->device == s->device;
-  for (int i = 0; same && i <= n.L(); ++i) same = n.d_[i] == s->nd.d[i];
+  bool same = h->G == s->G && n.L() == s->nd.L && h->device == s->device;
+  for (int i = 0; same && i < n.L(); ++i)
+    same = n.d_[i] == s->nd.lay[i].in && n.d_[i + 1] == s->nd.lay[i].out && (i < n.L() - 1 ? n.hidden_act() : n.out_act()) == s->nd.lay[i].act;
   if (!same) return ddrl_fail(DDRL_EINVAL, "the population's net has other dimensions, activations or another GPU than the snapshot");
   ON_DEVICE(s);
   const hipStream_t st = (hipStream_t)stream;
@@ -166,8 +171,8 @@ extern "C" int ddrl_snap_load_flat_dev(ddrl_snap_t *s, const float *d_flat, int6
   src.w = d_flat; src.agent = (size_t)ld; src.tiled = 0;
   int off = 0;
   for (int l = 0; l < s->nd.L; ++l) {
-    src.offw[l] = off; off += s->nd.d[l] * s->nd.d[l + 1];
-    src.offb[l] = off; off += s->nd.d[l + 1];
+    src.offw[l] = off; off += s->nd.lay[l].in * s->nd.lay[l].out;
+    src.offb[l] = off; off += s->nd.lay[l].out;
   }
   HIPCHK(snap_load_launch(&s->nd, s->img, &src, s->G, st));
   HIPCHK(hipEventRecord(s->loaded, st));
@@ -190,22 +195,24 @@ extern "C" int ddrl_snap_get_weights(ddrl_snap_t *s, double *flat) {
         const char *im = img.data() + g * n.stride;
         double *f = flat + (g0 + g) * n.np;
         for (int l = 0; l < n.L; ++l) {
-          const int K = n.d[l], N = n.d[l + 1];
+          const SnapLayer &y = n.lay[l];
+          const int K = y.in, N = y.out;
           for (int o = 0; o < N; ++o)
             for (int k = 0; k < K; ++k) {
-              const int strip = o >> 4, r = o & 15;
+              const char *rec = im + y.off + (size_t)(o >> 4) * y.rec;
+              const int r = o & 15;
               if (n.bits == 4) {
                 unsigned c;
-                memcpy(&c, im + n.woff[l] + snap_code_off(n.steps[l], strip, k >> 5, ((k >> 3) & 3) * 16 + r), 4);
-                const unsigned char e = (unsigned char)im[n.soff[l] + snap_scale_off(n.steps[l], strip, k >> 5, r)];
+                memcpy(&c, rec + (k >> 5) * 256 + (((k >> 3) & 3) * 16 + r) * 4, 4);
+                const unsigned char e = (unsigned char)rec[snap_scale_off(y.code, k >> 5, r)];
                 *f++ = std::ldexp(grid[(c >> (4 * (k & 7))) & 15], (int)e - 127);
               } else {
                 float v;
-                memcpy(&v, im + n.woff[l] + ((size_t)strip * n.steps[l] + (k >> 4)) * 1024 + ((((k >> 2) & 3) * 16 + r) * 4 + (k & 3)) * 4, 4);
+                memcpy(&v, rec + (k >> 4) * 1024 + ((((k >> 2) & 3) * 16 + r) * 4 + (k & 3)) * 4, 4);
                 *f++ = v;
               }
             }
-          for (int o = 0; o < N; ++o) { float v; memcpy(&v, im + n.boff[l] + o * 4, 4); *f++ = v; }
+          for (int o = 0; o < N; ++o) { float v; memcpy(&v, im + y.off + (size_t)(o >> 4) * y.rec + y.rec - 64 + (o & 15) * 4, 4); *f++ = v; }
         }
       }
     }
@@ -219,7 +226,7 @@ static int forward_on(ddrl_snap *s, const ddrl_snap_forward_args *a, hipStream_t
   if (a->n < 0) return ddrl_fail(DDRL_EINVAL, "n=%d < 0", a->n);
   if (a->n == 0) return DDRL_OK;
   if (!a->x || !a->out || off4(a->x) || off4(a->out)) return ddrl_fail(DDRL_EINVAL, "x / out NULL or misaligned");
-  const int64_t S = s->nd.d[0], A = s->nd.d[s->nd.L], n = a->n, G = s->G;
+  const int64_t S = s->nd.lay[0].in, A = s->nd.A, n = a->n, G = s->G;
   SnapForward p;
   p.G = s->G; p.n = a->n; p.per = 0; p.img = s->img;
   p.x = a->x; p.out = a->out; p.mask = a->mask;
@@ -247,7 +254,7 @@ extern "C" int ddrl_snap_forward(ddrl_snap_t *s, int n, const float *x, float *o
   if (!s || n < 0 || (n && (!x || !out))) return ddrl_fail(DDRL_EINVAL, "bad argument");
   if (n == 0) return DDRL_OK;
   ON_DEVICE(s);
-  const size_t nx = (size_t)s->G * n * s->nd.d[0] * 4, no = (size_t)s->G * n * s->nd.d[s->nd.L] * 4;
+  const size_t nx = (size_t)s->G * n * s->nd.lay[0].in * 4, no = (size_t)s->G * n * s->nd.A * 4;
   DevBuf b;
   if (b.get(up16(nx) + no) != hipSuccess) return ddrl_fail(DDRL_ENOMEM, "hipMalloc failed");
   ddrl_snap_forward_args a = {};
@@ -279,7 +286,7 @@ static int mixture_on(ddrl_snap *s, const ddrl_snap_mixture_args *a, hipStream_t
   const MixSpace w = mix_space(s, a->n, a->top_k);
   if (!a->workspace || ((uintptr_t)a->workspace & 15) || a->workspace_bytes < w.all)
     return ddrl_fail(DDRL_EINVAL, "workspace NULL, misaligned or under the %zu bytes of ddrl_snap_mixture_workspace", w.all);
-  const int S = s->nd.d[0], A = s->nd.d[s->nd.L];
+  const int S = s->nd.lay[0].in, A = s->nd.A;
   SnapMixture p;
   p.G = s->G; p.n = a->n; p.k = a->top_k; p.img = s->img;
   p.x = a->x; p.x_row = a->x_row == -1 ? S : a->x_row;
@@ -294,6 +301,7 @@ static int mixture_on(ddrl_snap *s, const ddrl_snap_mixture_args *a, hipStream_t
   p.idx = a->idx ? a->idx : (int *)(ws + w.idx);
   p.prob = a->prob ? a->prob : (float *)(ws + w.prob);
   p.y = a->y ? a->y : (float *)(ws + w.y);
+  p.ckey = (unsigned long long *)(ws + w.ckey); p.cidx = (int *)(ws + w.cidx); p.chunks = w.chunks;
   HIPCHK(snap_mixture_launch(&s->nd, &p, st));
   return DDRL_OK;
 }
@@ -310,7 +318,7 @@ extern "C" int ddrl_snap_mixture(ddrl_snap_t *s, int n, int top_k, const float *
   int rc = check_mix_shape(s, n, top_k);
   if (rc || n == 0) return rc;
   ON_DEVICE(s);
-  const size_t S = s->nd.d[0], A = s->nd.d[s->nd.L], G = s->G, places = (size_t)n * top_k;
+  const size_t S = s->nd.lay[0].in, A = s->nd.A, G = s->G, places = (size_t)n * top_k;
   const size_t sizes[8] = {n * S * 4, G * S * 4, router_b ? G * 4 : 0, allowed ? n * G : 0, n * A * 4, places * 4, places * 4, mix_space(s, n, top_k).all};
   size_t at[9] = {0};
   for (int i = 0; i < 8; ++i) at[i + 1] = at[i] + up16(sizes[i]);
@@ -354,7 +362,7 @@ extern "C" int ddrl_snap_mixture_grad_dev(ddrl_snap_t *s, const ddrl_snap_mixtur
   if (a->n && (!a->x || !a->idx || !a->prob || !a->y || !a->dout || off4(a->x) || off4(a->idx) || off4(a->prob) || off4(a->y) || off4(a->dout)))
     return ddrl_fail(DDRL_EINVAL, "x, idx, prob, y or dout NULL or misaligned");
   SnapGrad p;
-  p.G = s->G; p.n = a->n; p.k = a->top_k; p.S = s->nd.d[0]; p.A = s->nd.d[s->nd.L];
+  p.G = s->G; p.n = a->n; p.k = a->top_k; p.S = s->nd.lay[0].in; p.A = s->nd.A;
   p.x = a->x; p.x_row = a->x_row == -1 ? p.S : a->x_row;
   p.idx = a->idx; p.prob = a->prob; p.y = a->y;
   p.dout = a->dout; p.dout_row = a->dout_row == -1 ? p.A : a->dout_row;

@@ -8,52 +8,53 @@
 #define SNAP_MAXW 1024         // widest layer, as DDRL_WIDE_MAXW
 #define SNAP_MAXK 8            // DDRL_SNAP_MAX_TOP_K
 #define SNAP_LDS (160 * 1024)  // a CU's LDS
+#define SNAP_FEW 256           // places (rows x top_k) up to which a mixture answers each in a workgroup of its own
+#define SNAP_CHUNK 256         // agents a router workgroup looks at when there are few rows
 
-// An agent's net is one image of `stride` bytes, made for a matrix instruction whose A operand is 16 outputs (a "strip") by
-// one k-step of inputs, so that a wave's load is one contiguous piece of memory in lane order (lane = 16 q + r <-> output r of
-// the strip):
+// An agent's net is one image of `stride` bytes: its layers one after the other, a layer a row of records, one for 16 outputs
+// (a "strip"), made for a matrix instruction whose A operand is 16 outputs by one k-step of inputs, so that a wave's load is one
+// contiguous piece of memory in lane order (lane = 16 q + r <-> output r of the strip):
 //   32 bits: a k-step is 16 inputs, lane (r, q) holds inputs 4q .. 4q+3 as one float4: 1 KiB a step;
 //    4 bits: a k-step is 32 inputs, lane (r, q) holds inputs 8q .. 8q+7 as one dword of codes (lowest input in the lowest
-//            bits); four steps lie together (lane by lane 16 bytes, 1 KiB), the last steps % 4 ones each by itself (256 bytes);
-//            the scales are a byte each (E8M0: 2^(byte - 127)), [strip][step / 4][output][step % 4].
-// Outputs are padded to strips and inputs to k-steps with zeros.  Biases: fp32, padded with zeros.
-struct SnapDesc {
-  int L, bits, hact, oact;
-  int d[SNAP_MAXL + 1];
-  int in[SNAP_MAXL], out[SNAP_MAXL], A;                         // of layer l; of the net
-  int strips[SNAP_MAXL], steps[SNAP_MAXL];
-  unsigned woff[SNAP_MAXL], soff[SNAP_MAXL], boff[SNAP_MAXL];   // byte offsets in an image: weights, scales, biases
+//            bits): 256 bytes a step.  Behind the steps the scales, a byte each (E8M0: 2^(byte - 127)), [step / 4][output][step % 4].
+// A record ends with the 16 biases, fp32.  Outputs are padded to strips and inputs to k-steps with zeros.
+struct SnapLayer {
+  int in, out, strips, steps;
+  unsigned off, rec;                          // bytes: where the layer starts, a record
+  int act, code;                              // code: bytes of a record's steps
+};
+struct alignas(8) SnapDesc {                  // (the first argument of the kernels, which read it where it lies)
+  SnapLayer lay[SNAP_MAXL];
+  int L, bits, A, np;                         // layers; outputs of the net; parameters in the flat order
   unsigned stride;
-  int np;                                                       // parameters in the flat order
 };
 
 static inline void snap_build_desc(SnapDesc &n, int d0, const int *hidden, int nh, int dout, int hact, int oact, int bits) {
   n = SnapDesc();
-  n.L = nh + 1; n.bits = bits; n.hact = hact; n.oact = oact;
-  n.d[0] = d0;
-  for (int i = 0; i < nh; ++i) n.d[i + 1] = hidden[i];
-  n.d[nh + 1] = dout;
+  n.L = nh + 1; n.bits = bits; n.A = dout;
   unsigned off = 0;
   for (int l = 0; l < n.L; ++l) {
-    const int K = n.in[l] = n.d[l], N = n.out[l] = n.d[l + 1];
-    n.strips[l] = (N + 15) / 16;
-    n.steps[l] = bits == 4 ? (K + 31) / 32 : (K + 15) / 16;
-    n.woff[l] = off; off += (unsigned)n.strips[l] * n.steps[l] * (bits == 4 ? 256 : 1024);
-    n.soff[l] = off; if (bits == 4) off += (unsigned)n.strips[l] * ((n.steps[l] + 3) / 4) * 64;
-    n.boff[l] = off; off += (unsigned)n.strips[l] * 64;
+    SnapLayer &y = n.lay[l];
+    const int K = y.in = l ? hidden[l - 1] : d0, N = y.out = l < nh ? hidden[l] : dout;
+    y.act = l < nh ? hact : oact;
+    y.strips = (N + 15) / 16;
+    y.steps = bits == 4 ? (K + 31) / 32 : (K + 15) / 16;
+    y.code = y.steps * (bits == 4 ? 256 : 1024);
+    y.rec = (unsigned)y.code + (bits == 4 ? (y.steps + 3) / 4 * 64 : 0) + 64;
+    y.off = off; off += y.strips * y.rec;
     n.np += N * K + N;
   }
-  n.A = dout;
   n.stride = (off + 1023) / 1024 * 1024;
 }
-// where the code of (output n, 32-bit piece of 8 inputs (step, q)) of a 4-bit layer lies
-__host__ __device__ inline unsigned snap_code_off(int steps, int strip, int step, int lane) {
-  const int full = steps & ~3;
-  const unsigned at = (unsigned)strip * steps * 256;
-  return step < full ? at + (step >> 2) * 1024 + lane * 16 + (step & 3) * 4 : at + step * 256 + lane * 4;
-}
-__host__ __device__ inline unsigned snap_scale_off(int steps, int strip, int step, int r) {
-  return (unsigned)(strip * ((steps + 3) / 4) + (step >> 2)) * 64 + r * 4 + (step & 3);
+// where the scale of (output r of a strip, step) lies in a record
+__host__ __device__ inline unsigned snap_scale_off(int code, int step, int r) { return (unsigned)code + (step >> 2) * 64 + r * 4 + (step & 3); }
+
+// how many workgroups share a row's agents: with few rows as many as there are SNAP_CHUNKs, up to 16 (the lists are merged by
+// those who answer the places), else one
+static inline int snap_chunks(int G, int n, int k) {
+  if ((long long)n * k > SNAP_FEW) return 1;
+  const int c = (G + SNAP_CHUNK - 1) / SNAP_CHUNK;
+  return c > 16 ? 16 : c;
 }
 
 struct SnapForward {
@@ -73,6 +74,8 @@ struct SnapMixture {
   float *out; int64_t out_row;
   int *idx; float *prob; float *y;
   int *count;                         // [n] places of a row that are answered
+  unsigned long long *ckey; int *cidx;   // [n x chunks x k] each chunk's best, where the router's agents are spread over several workgroups
+  int chunks;
 };
 struct SnapGrad {
   int G, n, k, S, A;
