@@ -11,6 +11,7 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // The kernels' first argument in the kernel-argument memory itself: a layer is one scalar load there, whatever its number
 // (a run-time index into the by-value argument would make the compiler copy it to scratch memory)
@@ -22,16 +23,22 @@ __device__ __forceinline__ LayerOf layer_of(DescP nd, int l) {
   return LayerOf{y->in, y->out, y->strips, y->steps, y->act, y->code, y->off, y->rec};
 }
 
-__device__ __forceinline__ float act1(int t, float x) {
-  if (t == 2) return tanhf(x);
-  const float low = t == 1 ? 0.01f * x : t == 0 ? x : x != x ? x : 0.f;
-  return x > 0.f ? x : low;
+// linear and leaky-ReLU are max(x, slope x), ReLU is max(x, 0), with a maximum that keeps NaN
+__device__ __forceinline__ float act_one(int act, float x) {
+  if (act == 2) return tanhf(x);
+  return __builtin_elementwise_maximum(x, act == 3 ? 0.f : act == 1 ? 0.01f * x : x);
 }
-__device__ __forceinline__ f32x4 act4(int t, f32x4 x) {           // (one decision for four outputs)
-  if (t == 2) return f32x4{tanhf(x[0]), tanhf(x[1]), tanhf(x[2]), tanhf(x[3])};
-  if (t == 0) return x;
+__device__ __forceinline__ f32x4 act_four(int act, f32x4 x) {
+  if (act == 2) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] = x[j] > 0.f ? x[j] : t == 1 ? 0.01f * x[j] : x[j] != x[j] ? x[j] : 0.f;
+    for (int j = 0; j < 4; ++j) x[j] = tanhf(x[j]);
+  } else if (act == 3) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = __builtin_elementwise_maximum(x[j], 0.f);
+  } else if (act == 1) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = __builtin_elementwise_maximum(x[j], 0.01f * x[j]);
+  }
   return x;
 }
 
@@ -124,7 +131,7 @@ extern "C" hipError_t snap_load_launch(const SnapDesc *nd, char *img, const Snap
 // end.  And with R < 16 every lane finishes ONE output of the tile (bias, activation, the three parts) instead of a few lanes
 // finishing four: with few rows that, not the product, is most of the instructions.
 // ------------------------------------------------------------------------------------------------------------------------
-struct SnapLds { int second, image; };       // the inputs of layers 0, 2 lie in the first LDS buffer, those of 1, 3 in the second; behind them the image, where it is staged
+struct SnapLds { int second, image, first; };   // the inputs of layers 0, 2 lie in the first LDS buffer, those of 1, 3 in the second; behind them the image from byte `first` on, where it is staged
 
 template <int BITS, int R, int NT>
 struct SnapShape {
@@ -147,6 +154,13 @@ __device__ __forceinline__ void split3(float x, float (&v)[3]) {
   const float r1 = fabsf(x) < __uint_as_float(0x7f800000u) ? x - hi : 0.f;
   v[0] = x; v[1] = r1;
   v[2] = r1 - __uint_as_float(__float_as_uint(r1) & 0xffff0000u);
+}
+// what the upper halves leave
+__device__ __forceinline__ f32x4 rest4(f32x4 x) {
+  f32x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = x[j] - __uint_as_float(__float_as_uint(x[j]) & 0xffff0000u);
+  return r;
 }
 __device__ __forceinline__ unsigned two_tops(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
 
@@ -263,10 +277,10 @@ template <int BITS, int MT, int UB> struct SnapBlock {
 // What a wave works on: strips s .. s + MT - 1 of layer l
 struct Item { LayerOf y; int l, s; };
 template <int MT>
-__device__ __forceinline__ bool next_item(Item &it, DescP nd, int wave, int waves) {
+__device__ __forceinline__ bool next_item(Item &it, DescP nd, int end, int wave, int waves) {
   it.s += waves * MT;
   while (it.s >= it.y.strips) {
-    if (++it.l >= nd->L) return false;
+    if (++it.l >= end) return false;
     it.y = layer_of(nd, it.l);
     it.s = wave * MT;
   }
@@ -304,23 +318,26 @@ __device__ __forceinline__ void ahead_load(SnapAhead<BITS, R, MT, UB> &h, const 
   h.w.load(h.it.y, rec, 0, lane);
 }
 template <int BITS, int R, int MT, int UB>
-__device__ __forceinline__ void ahead_first(SnapAhead<BITS, R, MT, UB> &h, DescP nd, const char *img) {
+__device__ __forceinline__ void ahead_first(SnapAhead<BITS, R, MT, UB> &h, DescP nd, const char *img, int end) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   h.it.y = layer_of(nd, 0); h.it.l = 0; h.it.s = (wave - waves) * MT;
-  h.any = next_item<MT>(h.it, nd, wave, waves);
+  h.any = next_item<MT>(h.it, nd, end, wave, waves);
   if (h.any) ahead_load(h, img, lane);
 }
 
-// The inputs are in LDS, behind a barrier; `img`: the net's image, in memory (AHEAD: `h` comes from ahead_first, and whatever is
-// next, of the next layer too, is on its way while something is multiplied) or in LDS.  Ends with a barrier.
+// Layers from .. end - 1.  The inputs are in LDS, behind a barrier; `img`: the net's image, in memory (AHEAD: `h` comes from
+// ahead_first, and whatever is next, of the next layer too, is on its way while something is multiplied) or in LDS.  Ends with a
+// barrier.
 template <int BITS, int R, int NT, int MT, int UB, bool AHEAD, class Out>
-__device__ __forceinline__ void net_tile(SnapAhead<BITS, R, MT, UB> &h, DescP nd, const SnapLds &m, const char *img, char *lds, Out out) {
+__device__ __forceinline__ void net_layers(SnapAhead<BITS, R, MT, UB> &h, DescP nd, const SnapLds &m, const char *img, char *lds, int from, int end_, Out out) {
   using S = SnapShape<BITS, R, NT>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, c = lane & 15, q = lane >> 4;
   const int xrow = R == 16 ? c : (R == 4 ? c >> 2 : 0) + (BITS == 4 ? min(c & 3, 2) * S::T : 0);
+  LayerOf coming = layer_of(nd, from);
 #pragma unroll 1
-  for (int l = 0; l < nd->L; ++l) {
-    const LayerOf y = layer_of(nd, l);
+  for (int l = from; l < end_; ++l) {
+    const LayerOf y = coming;
+    coming = layer_of(nd, min(l + 1, SNAP_MAXL - 1));
     const int ldi = S::ld(y.in), ldo = S::ld(y.out);
     const char *xin = lds + (l & 1 ? m.second : 0) + xrow * ldi + q * 16;
     char *xout = lds + (l & 1 ? 0 : m.second);
@@ -360,7 +377,7 @@ __device__ __forceinline__ void net_tile(SnapAhead<BITS, R, MT, UB> &h, DescP nd
         }
         if (AHEAD) h.w = next;
       }
-      if (AHEAD && next_item<MT>(h.it, nd, wave, waves)) ahead_load(h, img, lane);
+      if (AHEAD && next_item<MT>(h.it, nd, end_, wave, waves)) ahead_load(h, img, lane);
       const bool odd = BITS == 4 && (y.strips & 1);            // the next layer's k-steps are 32 wide: zeros behind an odd last strip
       if constexpr (R < 16) {
         const int own = R > 1 ? 0 : BITS == 4 ? (c >> 2) & (MT - 1) : q & (MT - 1), at = BITS == 4 || R == 4 ? 4 * q + (c & 3) : c;
@@ -391,13 +408,15 @@ __device__ __forceinline__ void net_tile(SnapAhead<BITS, R, MT, UB> &h, DescP nd
             }
             if constexpr (BITS == 4) {                         // the parts lie in the lanes of a quad: smallest first
 #pragma unroll
-              for (int j = 0; j < 4; ++j) p[j] = (quad_lane<2>(p[j]) + quad_lane<1>(p[j])) + quad_lane<0>(p[j]);
+              for (int j = 0; j < 4; ++j) p[j] = quad_lane<0>((quad_lane<2>(p[j]) + quad_lane<1>(p[j])) + p[j]);
             }
             const int j = c & 3;
-            v = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
+            v = j & 1 ? p[1] : p[0];
+            const float v2 = j & 1 ? p[3] : p[2];
+            v = j & 2 ? v2 : v;
           }
           const int n = strip * 16 + at, t = R == 4 ? c >> 2 : 0;
-          v = act1(y.act, v + bias.v1[i]);
+          v = act_one(y.act, v + bias.v1[i]);
           v = n < y.out ? v : 0.f;
           const bool mine = strip < y.strips && (R == 4 || (BITS == 4 ? c < 4 * MT : q < MT));
           if (mine) {
@@ -423,7 +442,7 @@ __device__ __forceinline__ void net_tile(SnapAhead<BITS, R, MT, UB> &h, DescP nd
 #pragma unroll
             for (int tt = 0; tt < NT; ++tt) {
               const int t = 16 * tt + c;
-              f32x4 a = act4(y.act, acc[i][tt] + bias.v4[i]);
+              f32x4 a = act_four(y.act, acc[i][tt] + bias.v4[i]);
               if (end) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) a[j] = n0 + j < y.out ? a[j] : 0.f;
@@ -432,14 +451,20 @@ __device__ __forceinline__ void net_tile(SnapAhead<BITS, R, MT, UB> &h, DescP nd
 #pragma unroll
                 for (int j = 0; j < 4; ++j) if (n0 + j < y.out) out(t, n0 + j, a[j]);
               } else if constexpr (BITS == 4) {
-                float p[4][3];
+                f32x4 r = rest4(a);                          // NaN where a is not finite: rare enough to look for once
+                const float odd_one = __builtin_elementwise_maximum(__builtin_elementwise_maximum(r[0], r[1]), __builtin_elementwise_maximum(r[2], r[3]));
+                if (__any(odd_one != odd_one)) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) split3(a[j], p[j]);
+                  for (int j = 0; j < 4; ++j) r[j] = r[j] != r[j] ? 0.f : r[j];
+                }
+                const f32x4 lo = rest4(r);
+                char *o = xout + t * ldo + n0 * 2;
+                *(u32x2 *)o = u32x2{two_tops(a[0], a[1]), two_tops(a[2], a[3])};
+                *(u32x2 *)(o + S::T * ldo) = u32x2{two_tops(r[0], r[1]), two_tops(r[2], r[3])};
+                *(u32x2 *)(o + 2 * S::T * ldo) = u32x2{two_tops(lo[0], lo[1]), two_tops(lo[2], lo[3])};
+                if (odd && end) {
 #pragma unroll
-                for (int k = 0; k < 3; ++k) {
-                  char *o = xout + (k * S::T + t) * ldo + n0 * 2;
-                  *(u32x2 *)o = u32x2{two_tops(p[0][k], p[1][k]), two_tops(p[2][k], p[3][k])};
-                  if (odd && end) *(u32x2 *)(o + 32) = u32x2{0u, 0u};
+                  for (int k = 0; k < 3; ++k) *(u32x2 *)(o + k * S::T * ldo + 32) = u32x2{0u, 0u};
                 }
               } else *(f32x4 *)(xout + t * ldo + n0 * 4) = a;
             }
@@ -460,30 +485,46 @@ __device__ __forceinline__ void image_in(const char *img, char *lds, unsigned by
 }
 __device__ __forceinline__ void image_here() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// How a workgroup comes by its net: straight from memory as it goes (0), all of it staged in LDS (1), or all but the first layer
+// (2), which goes to registers meanwhile.  net_ask before the inputs are brought in, net_tile after them.
+template <int BITS, int R, int NT, int MT, int UB, int STAGE> struct SnapNet {
+  SnapAhead<BITS, R, MT, UB> h;
+  const char *img;
+  __device__ __forceinline__ void stage(DescP nd, const SnapLds &m, const char *image, char *lds) {      // once for a net
+    img = image;
+    if (STAGE) image_in(image + m.first, lds + m.image, nd->stride - m.first);
+  }
+  __device__ __forceinline__ void ask(DescP nd) { if (STAGE != 1) ahead_first(h, nd, img, STAGE ? 1 : nd->L); }     // for a tile
+  template <class Out>
+  __device__ __forceinline__ void tile(DescP nd, const SnapLds &m, char *lds, Out out) {
+    if (STAGE) image_here();
+    lds_barrier();
+    if (STAGE != 1) net_layers<BITS, R, NT, MT, UB, true>(h, nd, m, img, lds, 0, STAGE ? 1 : nd->L, out);
+    if (STAGE) net_layers<BITS, R, NT, MT, UB, false>(h, nd, m, lds + (m.image - m.first), lds, STAGE - 1, nd->L, out);
+  }
+};
+
 // ------------------------------------------------------------------------------------------------------------------------
 // Every agent's net on its rows
 // ------------------------------------------------------------------------------------------------------------------------
-template <int BITS, int R, int NT, int MT, int UB, bool STAGE>
-__global__ void __launch_bounds__(512)
+template <int BITS, int R, int NT, int MT, int UB, int STAGE>
+__global__ void __launch_bounds__(R == 16 && STAGE == 2 ? 1024 : 512)
 snap_forward_kernel(const SnapDesc nd_, const SnapLds m, const SnapForward p) {
   extern __shared__ __align__(16) char lds[];
   using S = SnapShape<BITS, R, NT>;
   const DescP nd = SNAP_DESC(nd_);
   const int g = blockIdx.x;
   if (p.mask && !p.mask[g]) return;
-  const char *img = p.img + (size_t)g * nd->stride;
-  if (STAGE) { image_in(img, lds + m.image, nd->stride); img = lds + m.image; }
+  SnapNet<BITS, R, NT, MT, UB, STAGE> net;
+  net.stage(nd, m, p.img + (size_t)g * nd->stride, lds);
   const int from = blockIdx.y * p.per, to = min(p.n, from + p.per);
 #pragma unroll 1
   for (int t0 = from; t0 < to; t0 += S::T) {
-    SnapAhead<BITS, R, MT, UB> h;
-    if (!STAGE) ahead_first(h, nd, img);
+    net.ask(nd);
     const float *x = p.x + g * p.x_agent + t0 * p.x_row;
     tile_in<BITS, R, NT>(nd->lay[0].in, lds, [&](int t) { return t0 + t < to ? x + t * p.x_row : (const float *)nullptr; });
-    if (STAGE) image_here();
-    lds_barrier();
     float *o = p.out + g * p.out_agent + t0 * p.out_row;
-    net_tile<BITS, R, NT, MT, UB, !STAGE>(h, nd, m, img, lds, [&](int t, int n, float v) { if (t0 + t < to) o[t * p.out_row + n] = v; });
+    net.tile(nd, m, lds, [&](int t, int n, float v) { if (t0 + t < to) o[t * p.out_row + n] = v; });
   }
 }
 
@@ -680,7 +721,7 @@ snap_router_kernel(const SnapMixture p, int S, int A, int ld) {
 // answered in.  The answers are stored past the XCD's own cache (agent scope); once they have arrived the counter may tell of
 // them.  Nothing else passes between workgroups, so no cache has to be written back or forgotten, and nobody waits.
 // ------------------------------------------------------------------------------------------------------------------------
-template <int BITS, int MT, int UB, bool STAGE>
+template <int BITS, int MT, int UB, int STAGE>
 __global__ void __launch_bounds__(512)
 snap_place_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
   extern __shared__ __align__(16) char lds[];
@@ -708,15 +749,12 @@ snap_place_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
     }
   }
   if (e < 0) return;
-  const char *img = p.img + (size_t)e * nd->stride;
-  SnapAhead<BITS, 1, MT, UB> h;
-  if (STAGE) { image_in(img, lds + m.image, nd->stride); img = lds + m.image; }
-  else ahead_first(h, nd, img);
+  SnapNet<BITS, 1, 1, MT, UB, STAGE> net;
+  net.stage(nd, m, p.img + (size_t)e * nd->stride, lds);
+  net.ask(nd);
   const float *x = p.x + row * p.x_row;
   tile_in<BITS, 1, 1>(nd->lay[0].in, lds, [&](int) { return x; });
-  if (STAGE) image_here();
-  lds_barrier();
-  net_tile<BITS, 1, 1, MT, UB, !STAGE>(h, nd, m, img, lds, [&](int, int n, float v) { __hip_atomic_store(y + n, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
+  net.tile(nd, m, lds, [&](int, int n, float v) { __hip_atomic_store(y + n, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
@@ -735,63 +773,122 @@ snap_place_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
-// The picked nets, many places: a workgroup answers, for one net, the places of a piece of idx that picked it, T at a time; the
+// Who picked a net, when there are many places: every 1024 places of idx sorted by the net they picked, in their order.  Lanes of a
+// wave with the same net find each other bit by bit; the waves take their turns at the nets' counters, so that a place's position
+// does not hang on who came first.  Places that picked nobody go to net G.
+// ------------------------------------------------------------------------------------------------------------------------
+#define SORT_BLOCK 1024
+__device__ __forceinline__ void sort_block(const int *__restrict__ idx, int block, int total, int G, int bits, int *__restrict__ sorted, int *__restrict__ start, char *lds) {
+  int *cnt = (int *)lds;                                   // [G + 1]
+  __shared__ int wsum[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = block * SORT_BLOCK + tid;
+  int e = i < total ? idx[i] : G;
+  for (int j = tid; j <= G; j += 1024) cnt[j] = 0;
+  e = e < 0 || e >= G ? G : e;
+  unsigned long long same = __ballot(i < total);
+  for (int b = 0; b < bits; ++b) {
+    const unsigned long long m = __ballot((e >> b) & 1);
+    same &= (e >> b) & 1 ? m : ~m;
+  }
+  const unsigned long long below = (1ull << lane) - 1ull;
+  const int rank = __popcll(same & below), n = __popcll(same), lead = __ffsll(same) - 1;
+  int base = 0;
+  for (int w = 0; w < 16; ++w) {
+    __syncthreads();
+    if (w == wave && i < total && lane == lead) base = atomicAdd(&cnt[e], n);
+  }
+  __syncthreads();
+  base = __shfl(base, lead < 0 ? 0 : lead) + rank;
+  // exclusive sums of the counters: a thread `per` of them, then the waves, then the block
+  const int per = (G + 1 + 1023) >> 10, e0 = tid * per;
+  int own = 0;
+  for (int j = 0; j < per; ++j) own += e0 + j <= G ? cnt[e0 + j] : 0;
+  int before = own;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) { const int o = __shfl_up(before, d); before += lane >= d ? o : 0; }
+  if (lane == 63) wsum[wave] = before;
+  __syncthreads();
+  before -= own;
+  for (int w = 0; w < wave; ++w) before += wsum[w];
+  __syncthreads();
+  for (int j = 0; j < per; ++j)
+    if (e0 + j <= G) { const int c = cnt[e0 + j]; cnt[e0 + j] = before; start[(int64_t)block * (G + 1) + e0 + j] = before; before += c; }
+  __syncthreads();
+  if (i < total) sorted[block * SORT_BLOCK + cnt[e] + base] = i;
+}
+extern "C" __global__ void __launch_bounds__(1024)
+snap_sort_kernel(const int *__restrict__ idx, int total, int G, int bits, int *__restrict__ sorted, int *__restrict__ start) {
+  extern __shared__ __align__(16) char lds[];
+  sort_block(idx, blockIdx.x, total, G, bits, sorted, start, lds);
+}
+// A net's places (or, e = G, those that picked nobody) in up to 256 blocks from b0 on, as one list
+struct Segments { int pre[257], at[256]; };
+__device__ __forceinline__ int segments_of(Segments &g, const int *start, int total, int G, int e, int b0, int blocks) {
+  // all threads of a workgroup of 256 or more; barriers inside
+  __shared__ int wsum[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __syncthreads();
+  int c = 0, sum = 0;
+  if (tid < 256) {
+    if (tid < blocks) {
+      const int *st = start + (int64_t)(b0 + tid) * (G + 1) + e;
+      const int from = st[0];
+      c = (e < G ? st[1] : min(SORT_BLOCK, total - (b0 + tid) * SORT_BLOCK)) - from;
+      g.at[tid] = (b0 + tid) * SORT_BLOCK + from;
+    }
+    sum = c;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) { const int o = __shfl_up(sum, d); sum += lane >= d ? o : 0; }
+    if (lane == 63) wsum[wave] = sum;
+  }
+  __syncthreads();
+  if (tid < 256) {
+    for (int w = 0; w < wave; ++w) sum += wsum[w];
+    g.pre[tid + 1] = sum;
+    if (tid == 0) g.pre[0] = 0;
+  }
+  __syncthreads();
+  return g.pre[256];
+}
+__device__ __forceinline__ int place_of(const Segments &g, const int *sorted, int i) {
+  int lo = 0;
+#pragma unroll
+  for (int d = 128; d; d >>= 1) lo += g.pre[lo + d] <= i ? d : 0;
+  return sorted[g.at[lo] + i - g.pre[lo]];
+}
+
+// ------------------------------------------------------------------------------------------------------------------------
+// The picked nets, many places: a workgroup answers, for one net, every gridDim.y-th tile of T of the places that picked it; the
 // rows are summed up as above.
 // ------------------------------------------------------------------------------------------------------------------------
-#define SNAP_LIST 1024
-template <int BITS, int R, int NT, int MT, int UB, bool STAGE>
+template <int BITS, int R, int NT, int MT, int UB, int STAGE>
 __global__ void __launch_bounds__(512)
-snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p, int piece) {
+snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
   extern __shared__ __align__(16) char lds[];
   using S = SnapShape<BITS, R, NT>;
-  __shared__ int list[SNAP_LIST + 2048], cnt, done[S::T];
+  __shared__ Segments seg;
+  __shared__ int list[S::T], done[S::T];
   const DescP nd = SNAP_DESC(nd_);
-  const int tid = threadIdx.x, A = nd->A, total = p.n * p.k, threads = blockDim.x, e = blockIdx.x;
-  int from = blockIdx.y * piece;
-  const int to = min(total, from + piece);
-  const char *img = p.img + (size_t)e * nd->stride;
+  const int tid = threadIdx.x, A = nd->A, threads = blockDim.x, e = blockIdx.x;
+  SnapNet<BITS, R, NT, MT, UB, STAGE> net;
   bool staged = false;
-  while (from < to) {
-    __syncthreads();
-    if (tid == 0) cnt = 0;
-    __syncthreads();
-    for (;;) {                                             // 4 places a thread and round
-      int v[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { const int i = from + j * threads + tid; v[j] = i < to ? p.idx[i] : -1; }
-      int mine = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) mine += v[j] == e;
-      if (mine) {
-        int at = atomicAdd(&cnt, mine);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) if (v[j] == e) list[at++] = from + j * threads + tid;
-      }
-      from += 4 * threads;
-      if (from >= to) break;
+  for (int b0 = 0; b0 < p.blocks; b0 += 256) {
+    const int have = segments_of(seg, p.start, p.n * p.k, p.G, e, b0, min(256, p.blocks - b0));
+    for (int i0 = blockIdx.y * S::T; i0 < have; i0 += gridDim.y * S::T) {
+      if (!staged) { net.stage(nd, m, p.img + (size_t)e * nd->stride, lds); staged = true; }
+      net.ask(nd);
+      if (tid < S::T) list[tid] = i0 + tid < have ? place_of(seg, p.sorted, i0 + tid) : -1;
       __syncthreads();
-      const int have = cnt;
-      __syncthreads();
-      if (have > SNAP_LIST) break;
-    }
-    __syncthreads();
-    const int have = cnt;
-    if (STAGE && have && !staged) { image_in(img, lds + m.image, nd->stride); img = lds + m.image; staged = true; }
-    for (int i0 = 0; i0 < have; i0 += S::T) {
-      SnapAhead<BITS, R, MT, UB> h;
-      if (!STAGE) ahead_first(h, nd, img);
-      tile_in<BITS, R, NT>(nd->lay[0].in, lds, [&](int t) { return i0 + t < have ? p.x + (int64_t)(list[i0 + t] / p.k) * p.x_row : (const float *)nullptr; });
-      if (STAGE) image_here();
-      lds_barrier();
-      net_tile<BITS, R, NT, MT, UB, !STAGE>(h, nd, m, img, lds, [&](int t, int n, float v) {
-        if (i0 + t < have) __hip_atomic_store(p.y + (int64_t)list[i0 + t] * A + n, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      tile_in<BITS, R, NT>(nd->lay[0].in, lds, [&](int t) { return list[t] >= 0 ? p.x + (int64_t)(list[t] / p.k) * p.x_row : (const float *)nullptr; });
+      net.tile(nd, m, lds, [&](int t, int n, float v) {
+        if (list[t] >= 0) __hip_atomic_store(p.y + (int64_t)list[t] * A + n, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       });
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       if (tid < S::T) {
         int row = -1;
-        if (i0 + tid < have) {
-          const int r = list[i0 + tid] / p.k;
+        if (list[tid] >= 0) {
+          const int r = list[tid] / p.k;
           int want = 0;
           for (int j = 0; j < p.k; ++j) want += p.idx[r * p.k + j] >= 0;
           if (__hip_atomic_fetch_add(p.count + r, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == want - 1) row = r;
@@ -814,70 +911,91 @@ snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p, in
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
-// The router's gradient.  One workgroup per agent (and one more for the places that picked nobody): it walks idx in order and,
-// for every 256 places that are its own, one thread each takes the place's dlogit, then all sum dlogit x over them: thread
-// (u, s) over the places u, u + parts, .. of input s, in fp64 (an agent may be picked by every row).
+// The router's gradient.  16 lanes take the dlogit of a place (a lane the outputs a, a + 16, ..).
+// Few places: one launch, a workgroup per agent looks through idx itself, 256 places at once, and sums dlogit x over its own:
+// thread (u, s) over the collected places u, u + parts, .. of input s, and the parts in their order.
+// Many: a first launch takes all dlogits and, in other workgroups, sorts the places by agent; in a second one a workgroup per agent
+// sums over the places that picked it, in their order, a wave every fourth of them and a lane an input.  Few agents: several
+// workgroups each, a run of sorted blocks every one; their sums go to the workspace, and the last of them adds all, in order.
+// Sums over rows are in fp64 (an agent may be picked by every row).
 // ------------------------------------------------------------------------------------------------------------------------
-extern "C" __global__ void __launch_bounds__(256)
-snap_grad_kernel(const SnapGrad p) {
-  __shared__ int list[512], wsum[4];
-  __shared__ float dl[512];
-  __shared__ double part[256];
-  const int e = blockIdx.x, tid = threadIdx.x, total = p.n * p.k, S = p.S, A = p.A;
-  if (e == p.G) {                                          // dy of places that picked nobody
-    if (!p.dy) return;
-    for (int i = tid; i < total; i += 256) {
-      const int v = p.idx[i];
-      if (v >= 0 && v < p.G) continue;
-      for (int a = 0; a < A; ++a) p.dy[(int64_t)i * A + a] = 0.f;
-    }
-    return;
+__device__ __forceinline__ float sum_of_16(float v) {
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, true));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, true));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, true));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xf, 0xf, true));
+  return v;
+}
+// dlogit of a place, in all of its 16 lanes (a0 = 0 .. 15), and dy; one that picked nobody: 0
+template <int KM>
+__device__ __forceinline__ float dlogit_of(const SnapGrad &p, int place, int a0) {
+  const int r = place / p.k, j = place - r * p.k, A = p.A;
+  const float *dout = p.dout + (int64_t)r * p.dout_row, *y = p.y + (int64_t)r * p.k * A;
+  float dot[KM], pr[KM];
+  unsigned picked = 0;                                     // places that picked nobody may hold anything
+#pragma unroll
+  for (int v = 0; v < KM; ++v) {
+    const int at = r * p.k + min(v, p.k - 1), ev = p.idx[at];
+    pr[v] = p.prob[at];
+    picked |= (v < p.k && ev >= 0 && ev < p.G) << v;
+    dot[v] = 0.f;
   }
+  for (int a = a0; a < A; a += 16) {
+    const float d = dout[a];
+#pragma unroll
+    for (int v = 0; v < KM; ++v) dot[v] = fmaf(y[min(v, p.k - 1) * A + a], d, dot[v]);
+  }
+  float all = 0.f, own = 0.f, pj = 0.f;
+#pragma unroll
+  for (int v = 0; v < KM; ++v) {
+    const float d = sum_of_16(dot[v]);
+    all = picked >> v & 1 ? fmaf(pr[v], d, all) : all;
+    if (v == j) { own = d; pj = picked >> v & 1 ? pr[v] : 0.f; }
+  }
+  if (p.dy) for (int a = a0; a < A; a += 16) p.dy[(int64_t)place * A + a] = picked >> j & 1 ? pj * dout[a] : 0.f;
+  return picked >> j & 1 ? pj * (own - all) : 0.f;
+}
+
+template <int KM>
+__global__ void __launch_bounds__(256)
+snap_grad_few_kernel(const SnapGrad p) {
+  __shared__ int list[256], wsum[4];
+  __shared__ float dl[256];
+  __shared__ double part[256];
+  const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = p.S, total = p.n * p.k;
   const int s0 = S < 256 ? S : 256, parts = 256 / s0, u = tid / s0, sx = tid - u * s0;
   double acc[4] = {0., 0., 0., 0.}, bacc = 0.;             // S <= 1024
-  int from = 0, have = 0;
-  while (from < total) {
-    while (from < total && have <= 256) {                  // ordered: wave by wave, lane by lane
-      const int i = from + tid;
-      const bool mine = i < total && p.idx[i] == e;
-      const unsigned long long b = __ballot(mine);
-      const int w = tid >> 6, lane = tid & 63;
-      if (lane == 0) wsum[w] = __popcll(b);
-      __syncthreads();
-      int at = have;
-      for (int j = 0; j < w; ++j) at += wsum[j];
-      if (mine) list[at + __popcll(b & ((1ull << lane) - 1ull))] = i;
-      have += wsum[0] + wsum[1] + wsum[2] + wsum[3];
-      from += 256;
-      __syncthreads();
-    }
-    for (int i = tid; i < have; i += 256) {
-      const int place = list[i], r = place / p.k, j = place - r * p.k;
-      const float *dout = p.dout + (int64_t)r * p.dout_row;
-      float all = 0.f, own = 0.f;
-      for (int v = 0; v < p.k; ++v) {
-        const int ev = p.idx[r * p.k + v];
-        if (ev < 0 || ev >= p.G) continue;
-        float dot = 0.f;
-        const float *y = p.y + ((int64_t)r * p.k + v) * A;
-        for (int a = 0; a < A; ++a) dot = fmaf(y[a], dout[a], dot);
-        all = fmaf(p.prob[r * p.k + v], dot, all);
-        if (v == j) own = dot;
-      }
-      const float pr = p.prob[place];
-      dl[i] = pr * (own - all);
-      if (p.dy) for (int a = 0; a < A; ++a) p.dy[(int64_t)place * A + a] = pr * dout[a];
+  for (int from = 0; from < total; from += 256) {
+    const int i = from + tid;
+    const int v = i < total ? p.idx[i] : -1;
+    // (agent 0's workgroup also looks after the places that picked nobody: their dy)
+    const bool mine = i < total && (v == e || (e == 0 && p.dy && (v < 0 || v >= p.G)));
+    const unsigned long long b = __ballot(mine);
+    if (lane == 0) wsum[wave] = __popcll(b);
+    __syncthreads();
+    int at = 0;
+    for (int w = 0; w < wave; ++w) at += wsum[w];
+    if (mine) list[at + __popcll(b & ((1ull << lane) - 1ull))] = i;
+    const int have = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+    __syncthreads();
+    if (!have) continue;
+    for (int m = tid >> 4; m < have; m += 16) {
+      const float d = dlogit_of<KM>(p, list[m], tid & 15);
+      if ((tid & 15) == 0) dl[m] = d;
     }
     __syncthreads();
-    if (u < parts)
-      for (int i = u; i < have; i += parts) {
-        const float *x = p.x + (int64_t)(list[i] / p.k) * p.x_row;
-        const double d = dl[i];
+    if (u < parts) {
+#pragma unroll 4
+      for (int m = u; m < have; m += parts) {
+        const float *x = p.x + (int64_t)(list[m] / p.k) * p.x_row;
+        const int pick = p.idx[list[m]];
+        const double d = dl[m];
+        if (pick != e) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) { const int s = sx + 256 * j; if (s < S && (j == 0 || s0 == 256)) acc[j] = fma(d, (double)x[s], acc[j]); }
         if (sx == 0) bacc += d;
       }
-    have = 0;
+    }
     __syncthreads();
   }
 #pragma unroll
@@ -885,10 +1003,11 @@ snap_grad_kernel(const SnapGrad p) {
     if (256 * j >= S) break;
     part[tid] = acc[j];
     __syncthreads();
-    if (u == 0 && sx + 256 * j < S) {
+    const int s = sx + 256 * j;
+    if (u == 0 && s < S) {
       double v = 0.;
       for (int i = 0; i < parts; ++i) v += part[i * s0 + sx];
-      p.dw[(int64_t)e * p.dw_row + sx + 256 * j] = (float)v;
+      p.dw[(int64_t)e * p.dw_row + s] = (float)v;
     }
     __syncthreads();
   }
@@ -903,6 +1022,87 @@ snap_grad_kernel(const SnapGrad p) {
   }
 }
 
+// workgroups 0 .. blocks - 1 sort, the others take 64 dlogits each
+template <int KM>
+__global__ void __launch_bounds__(1024)
+snap_grad_first_kernel(const SnapGrad p, int bits) {
+  extern __shared__ __align__(16) char lds[];
+  const int tid = threadIdx.x, total = p.n * p.k;
+  if ((int)blockIdx.x < p.blocks) {
+    if (p.sums && blockIdx.x == 0) for (int e = tid; e < p.G; e += 1024) p.done[e] = 0;
+    sort_block(p.idx, blockIdx.x, total, p.G, bits, p.sorted, p.start, lds);
+    return;
+  }
+  const int place = (blockIdx.x - p.blocks) * 64 + (tid >> 4);
+  if (place >= total) return;                              // (16 lanes together)
+  const float d = dlogit_of<KM>(p, place, tid & 15);
+  if ((tid & 15) == 0) p.dlogit[place] = d;
+}
+
+template <int SJ>                                          // 64 SJ inputs
+__global__ void __launch_bounds__(256)
+snap_grad_sum_kernel(const SnapGrad p) {
+  __shared__ Segments seg;
+  __shared__ int rows[256], last;
+  __shared__ float dl[256];
+  __shared__ double part[4][64];
+  const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), S = p.S;
+  double acc[SJ], bacc = 0.;
+#pragma unroll
+  for (int j = 0; j < SJ; ++j) acc[j] = 0.;
+  const int b_from = blockIdx.y * p.piece, b_to = min(p.blocks, b_from + p.piece);
+  for (int b0 = b_from; b0 < b_to; b0 += 256) {
+    const int have = segments_of(seg, p.start, p.n * p.k, p.G, e, b0, min(256, b_to - b0));
+    for (int i0 = 0; i0 < have; i0 += 256) {
+      const int now = min(256, have - i0);
+      if (tid < now) {
+        const int place = place_of(seg, p.sorted, i0 + tid);
+        rows[tid] = place / p.k;
+        dl[tid] = p.dlogit[place];
+      }
+      __syncthreads();
+#pragma unroll 8
+      for (int i = wave; i < now; i += 4) {
+        const double d = dl[i];
+        const float *x = p.x + (int64_t)rows[i] * p.x_row;
+#pragma unroll
+        for (int j = 0; j < SJ; ++j) acc[j] = fma(d, (double)x[min(64 * j + lane, S - 1)], acc[j]);
+        bacc += d;
+      }
+      __syncthreads();
+    }
+  }
+  double *ws = p.sums ? p.sums + ((size_t)blockIdx.y * p.G + e) * (S + 1) : nullptr;
+#pragma unroll
+  for (int j = 0; j < SJ + 1; ++j) {                       // the waves, in order; row SJ: the bias, column S of the workspace's rows
+    if (j == SJ && !p.db) break;
+    part[wave][lane] = j < SJ ? acc[j < SJ ? j : 0] : bacc;
+    __syncthreads();
+    const int s = j < SJ ? 64 * j + lane : S;
+    if (wave == 0 && (j < SJ ? s < S : lane == 0)) {
+      const double v = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
+      if (ws) __hip_atomic_store(ws + s, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      else if (s < S) p.dw[(int64_t)e * p.dw_row + s] = (float)v;
+      else p.db[e] = (float)v;
+    }
+    __syncthreads();
+  }
+  if (!ws) return;
+  // whoever is last of an agent's workgroups adds their sums (stored past the XCD's cache, told of once arrived)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) last = __hip_atomic_fetch_add(p.done + e, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.y - 1;
+  __syncthreads();
+  if (!last) return;
+  for (int s = tid; s < S + (p.db ? 1 : 0); s += 256) {
+    double v = 0.;
+#pragma unroll 8
+    for (int j = 0; j < (int)gridDim.y; ++j)
+      v += __hip_atomic_load(p.sums + ((size_t)j * p.G + e) * (S + 1) + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (s < S) p.dw[(int64_t)e * p.dw_row + s] = (float)v; else p.db[e] = (float)v;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------------------
 // launches
 // ------------------------------------------------------------------------------------------------------------------------
@@ -911,11 +1111,24 @@ static int most_strips(const SnapDesc &nd) {
   for (int l = 0; l < nd.L; ++l) most = nd.lay[l].strips > most ? nd.lay[l].strips : most;
   return most;
 }
-#define SNAP_STAGE (64 * 1024)      // images up to here are staged: two workgroups and more of them fit a CU
-template <int BITS, int R, int NT, int MT, int UB, bool STAGE>
-static hipError_t forward_run(const SnapDesc &nd, SnapForward p, hipStream_t st) {
+static int waves_for(const SnapDesc &nd, int mt, int most) {
+  const int waves = (most_strips(nd) + mt - 1) / mt;
+  return waves > most ? most : waves;
+}
+// the LDS of a kernel, and where in it what lies
+template <int BITS, int R, int NT, int STAGE>
+static int lds_for(const SnapDesc &nd, SnapLds &m) {
+  const int x = SnapShape<BITS, R, NT>::bytes(nd, m);
+  m.first = STAGE == 2 ? nd.lay[1].off & ~1023 : 0;
+  return x + (STAGE ? nd.stride - m.first : 0);
+}
+template <int BITS, int R, int NT, int STAGE>
+static bool fits(const SnapDesc &nd, int most) { SnapLds m; return lds_for<BITS, R, NT, STAGE>(nd, m) <= most; }
+
+template <int BITS, int R, int NT, int MT, int UB, int STAGE>
+static hipError_t forward_run(const SnapDesc &nd, SnapForward p, int most_waves, hipStream_t st) {
   SnapLds m;
-  const int lds = SnapShape<BITS, R, NT>::bytes(nd, m) + (STAGE ? nd.stride : 0), T = R * NT;
+  const int lds = lds_for<BITS, R, NT, STAGE>(nd, m), T = R * NT;
   static LdsConfig cfg;
   const auto kernel = snap_forward_kernel<BITS, R, NT, MT, UB, STAGE>;
   hipError_t e = ddrl_set_lds(kernel, lds, cfg);
@@ -925,31 +1138,34 @@ static hipError_t forward_run(const SnapDesc &nd, SnapForward p, hipStream_t st)
   if (chunks > tiles) chunks = tiles;
   const int per = (tiles + chunks - 1) / chunks;
   p.per = per * T;
-  int waves = (most_strips(nd) + MT - 1) / MT;
-  waves = waves > 8 ? 8 : waves;
-  hipLaunchKernelGGL(kernel, dim3(p.G, (tiles + per - 1) / per), dim3(waves * 64), lds, st, nd, m, p);
+  hipLaunchKernelGGL(kernel, dim3(p.G, (tiles + per - 1) / per), dim3(waves_for(nd, MT, most_waves) * 64), lds, st, nd, m, p);
   return hipGetLastError();
 }
-template <int BITS, int R, int NT>
-static bool fits(const SnapDesc &nd, int more) { SnapLds m; return SnapShape<BITS, R, NT>::bytes(nd, m) + more <= SNAP_LDS; }
 
+#define SNAP_HALF (SNAP_LDS / 2)      // two workgroups a CU: one computes while the other's net arrives
 extern "C" hipError_t snap_forward_launch(const SnapDesc *nd, const SnapForward *p, hipStream_t st) {
-  const int img = nd->stride;
-  const bool stage = img <= SNAP_STAGE;
+  const bool deep = nd->L > 1;
   if (nd->bits == 4) {
-    if (p->n > 16 && stage && fits<4, 16, 2>(*nd, img)) return forward_run<4, 16, 2, 2, 4, true>(*nd, *p, st);
-    if (p->n > 4 && stage && fits<4, 16, 1>(*nd, img)) return forward_run<4, 16, 1, 2, 4, true>(*nd, *p, st);
-    if (p->n > 4 && fits<4, 16, 1>(*nd, 0)) return forward_run<4, 16, 1, 4, 4, false>(*nd, *p, st);
-    if (p->n > 1 && stage && fits<4, 4, 1>(*nd, img)) return forward_run<4, 4, 1, 2, 4, true>(*nd, *p, st);
-    if (p->n > 1) return forward_run<4, 4, 1, 2, 4, false>(*nd, *p, st);
-    if (stage && fits<4, 1, 1>(*nd, img)) return forward_run<4, 1, 1, 2, 4, true>(*nd, *p, st);
-    return forward_run<4, 1, 1, 2, 4, false>(*nd, *p, st);
+    if (p->n > 4) {
+      if (fits<4, 16, 1, 1>(*nd, SNAP_HALF)) return forward_run<4, 16, 1, 2, 4, 1>(*nd, *p, 8, st);
+      if (deep && fits<4, 16, 1, 2>(*nd, SNAP_LDS)) return forward_run<4, 16, 1, 2, 4, 2>(*nd, *p, 16, st);
+      if (fits<4, 16, 1, 0>(*nd, SNAP_LDS)) return forward_run<4, 16, 1, 4, 4, 0>(*nd, *p, 8, st);
+    }
+    if (p->n > 1) {
+      if (fits<4, 4, 1, 1>(*nd, SNAP_HALF)) return forward_run<4, 4, 1, 2, 4, 1>(*nd, *p, 8, st);
+      if (deep && fits<4, 4, 1, 2>(*nd, SNAP_HALF)) return forward_run<4, 4, 1, 2, 4, 2>(*nd, *p, 8, st);
+      return forward_run<4, 4, 1, 2, 4, 0>(*nd, *p, 8, st);
+    }
+    if (fits<4, 1, 1, 1>(*nd, SNAP_HALF)) return forward_run<4, 1, 1, 2, 4, 1>(*nd, *p, 8, st);
+    if (deep && fits<4, 1, 1, 2>(*nd, SNAP_HALF)) return forward_run<4, 1, 1, 2, 4, 2>(*nd, *p, 8, st);
+    return forward_run<4, 1, 1, 2, 4, 0>(*nd, *p, 8, st);
   }
-  if (p->n > 16 && fits<32, 16, 2>(*nd, 0)) return forward_run<32, 16, 2, 2, 4, false>(*nd, *p, st);
-  if (p->n > 1 && stage && fits<32, 16, 1>(*nd, img)) return forward_run<32, 16, 1, 2, 4, true>(*nd, *p, st);
-  if (p->n > 1) return forward_run<32, 16, 1, 2, 4, false>(*nd, *p, st);
-  if (stage && fits<32, 1, 1>(*nd, img)) return forward_run<32, 1, 1, 2, 4, true>(*nd, *p, st);
-  return forward_run<32, 1, 1, 2, 4, false>(*nd, *p, st);
+  if (p->n > 1) {
+    if (fits<32, 16, 1, 1>(*nd, SNAP_HALF)) return forward_run<32, 16, 1, 2, 4, 1>(*nd, *p, 8, st);
+    return forward_run<32, 16, 1, 2, 4, 0>(*nd, *p, 8, st);
+  }
+  if (fits<32, 1, 1, 1>(*nd, SNAP_HALF)) return forward_run<32, 1, 1, 2, 4, 1>(*nd, *p, 8, st);
+  return forward_run<32, 1, 1, 2, 4, 0>(*nd, *p, 8, st);
 }
 
 template <int KM>
@@ -965,59 +1181,97 @@ static hipError_t router_run(const SnapMixture &p, int S, int A, hipStream_t st)
   hipLaunchKernelGGL(snap_router_kernel<KM>, dim3((p.n + 15) / 16, p.chunks), dim3(waves * 64), lds, st, p, S, A, ld);
   return hipGetLastError();
 }
-static int waves_for(const SnapDesc &nd, int mt) {
-  const int waves = (most_strips(nd) + mt - 1) / mt;
-  return waves > 8 ? 8 : waves;
-}
-template <int BITS, int MT, int UB, bool STAGE>
+template <int BITS, int MT, int UB, int STAGE>
 static hipError_t place_run(const SnapDesc &nd, const SnapMixture &p, hipStream_t st) {
   SnapLds m;
-  const int lds = SnapShape<BITS, 1, 1>::bytes(nd, m) + (STAGE ? nd.stride : 0);
+  const int lds = lds_for<BITS, 1, 1, STAGE>(nd, m);
   static LdsConfig cfg;
   const auto kernel = snap_place_kernel<BITS, MT, UB, STAGE>;
   hipError_t e = ddrl_set_lds(kernel, lds, cfg);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kernel, dim3(p.n * p.k), dim3(waves_for(nd, MT) * 64), lds, st, nd, m, p);
+  hipLaunchKernelGGL(kernel, dim3(p.n * p.k), dim3(waves_for(nd, MT, 8) * 64), lds, st, nd, m, p);
   return hipGetLastError();
 }
-template <int BITS, int R, int NT, int MT, int UB, bool STAGE>
+template <int BITS, int R, int NT, int MT, int UB, int STAGE>
 static hipError_t experts_run(const SnapDesc &nd, const SnapMixture &p, hipStream_t st) {
   SnapLds m;
-  const int lds = SnapShape<BITS, R, NT>::bytes(nd, m) + (STAGE ? nd.stride : 0);
+  const int lds = lds_for<BITS, R, NT, STAGE>(nd, m);
   static LdsConfig cfg;
   const auto kernel = snap_experts_kernel<BITS, R, NT, MT, UB, STAGE>;
   hipError_t e = ddrl_set_lds(kernel, lds, cfg);
   if (e != hipSuccess) return e;
-  int waves = waves_for(nd, MT);
+  int waves = waves_for(nd, MT, 8);
   waves = waves < 4 ? 4 : waves;
-  const int total = p.n * p.k, pieces = (1024 + p.G - 1) / p.G;
-  const int piece = ddrl_roundup((total + pieces - 1) / pieces, 1024);
-  hipLaunchKernelGGL(kernel, dim3(p.G, (total + piece - 1) / piece), dim3(waves * 64), lds, st, nd, m, p, piece);
+  // Several workgroups a net, each every share-th of its tiles: a router prefers some nets, and a net's tiles one after the other
+  // are what a pass then waits for (256 nets, 4096 rows, top 2: 53 us with 2 workgroups a net, 25 us with 8); a workgroup that
+  // finds no tile is over after two reads.
+  const int64_t total = (int64_t)p.n * p.k, T = R * NT;
+  int64_t share = (2048 + p.G - 1) / p.G;
+  const int64_t tiles = (total + T - 1) / T;
+  if (share > tiles) share = tiles;
+  hipLaunchKernelGGL(kernel, dim3(p.G, (unsigned)share), dim3(waves * 64), lds, st, nd, m, p);
+  return hipGetLastError();
+}
+static int sort_bits(int G) {
+  int bits = 1;
+  while ((1ll << bits) <= G) ++bits;
+  return bits;
+}
+static hipError_t sort_run(const int *idx, int total, int G, int *sorted, int *start, hipStream_t st) {
+  const size_t lds = (size_t)(G + 1) * 4;
+  static LdsConfig cfg;
+  hipError_t e = ddrl_set_lds(snap_sort_kernel, lds, cfg);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(snap_sort_kernel, dim3((total + SORT_BLOCK - 1) / SORT_BLOCK), dim3(1024), lds, st, idx, total, G, sort_bits(G), sorted, start);
   return hipGetLastError();
 }
 
-#define SNAP_STATIC_LDS 13312        // snap_experts_kernel's list and flags
+#define SNAP_STATIC_LDS 2560         // snap_experts_kernel's lists
 extern "C" hipError_t snap_mixture_launch(const SnapDesc *nd, const SnapMixture *p, hipStream_t st) {
   const int S = nd->lay[0].in, A = nd->A;
   hipError_t e = p->k == 1 ? router_run<1>(*p, S, A, st) : p->k == 2 ? router_run<2>(*p, S, A, st) : p->k <= 4 ? router_run<4>(*p, S, A, st)
                                                                                                               : router_run<8>(*p, S, A, st);
   if (e != hipSuccess) return e;
-  const int total = p->n * p->k, img = nd->stride;
-  const bool stage = img <= SNAP_STAGE;
+  const int total = p->n * p->k, left = SNAP_LDS - SNAP_STATIC_LDS;
+  const bool deep = nd->L > 1;
   if (total <= SNAP_FEW) {
-    if (nd->bits == 4) return stage ? place_run<4, 2, 4, true>(*nd, *p, st) : place_run<4, 2, 4, false>(*nd, *p, st);
-    return stage ? place_run<32, 2, 4, true>(*nd, *p, st) : place_run<32, 2, 4, false>(*nd, *p, st);
+    if (nd->bits == 4)
+      return fits<4, 1, 1, 1>(*nd, SNAP_HALF) ? place_run<4, 2, 4, 1>(*nd, *p, st)
+             : deep && fits<4, 1, 1, 2>(*nd, SNAP_LDS - 1024) ? place_run<4, 2, 4, 2>(*nd, *p, st) : place_run<4, 2, 4, 0>(*nd, *p, st);
+    return fits<32, 1, 1, 1>(*nd, SNAP_HALF) ? place_run<32, 2, 4, 1>(*nd, *p, st) : place_run<32, 2, 4, 0>(*nd, *p, st);
   }
+  if ((e = sort_run(p->idx, total, p->G, p->sorted, p->start, st)) != hipSuccess) return e;
   if (nd->bits == 4) {
-    if (stage && fits<4, 16, 1>(*nd, SNAP_STATIC_LDS + img)) return experts_run<4, 16, 1, 2, 4, true>(*nd, *p, st);
-    if (fits<4, 16, 1>(*nd, SNAP_STATIC_LDS)) return experts_run<4, 16, 1, 4, 4, false>(*nd, *p, st);
-    return experts_run<4, 4, 1, 2, 4, false>(*nd, *p, st);
+    if (fits<4, 16, 1, 1>(*nd, left)) return experts_run<4, 16, 1, 2, 4, 1>(*nd, *p, st);
+    if (fits<4, 16, 1, 0>(*nd, left)) return experts_run<4, 16, 1, 4, 4, 0>(*nd, *p, st);
+    return experts_run<4, 4, 1, 2, 4, 0>(*nd, *p, st);
   }
-  if (stage && fits<32, 16, 1>(*nd, SNAP_STATIC_LDS + img)) return experts_run<32, 16, 1, 2, 4, true>(*nd, *p, st);
-  return experts_run<32, 16, 1, 2, 4, false>(*nd, *p, st);
+  if (fits<32, 16, 1, 1>(*nd, left)) return experts_run<32, 16, 1, 1, 4, 1>(*nd, *p, st);
+  if (fits<32, 16, 1, 0>(*nd, left)) return experts_run<32, 16, 1, 1, 4, 0>(*nd, *p, st);
+  return experts_run<32, 1, 1, 2, 4, 0>(*nd, *p, st);
 }
 
-extern "C" hipError_t snap_grad_launch(const SnapGrad *p, hipStream_t st) {
-  hipLaunchKernelGGL(snap_grad_kernel, dim3(p->G + (p->dy ? 1 : 0)), dim3(256), 0, st, *p);
+template <int KM>
+static hipError_t grad_first_run(const SnapGrad &p, hipStream_t st) {
+  if (!p.sorted) {
+    hipLaunchKernelGGL(snap_grad_few_kernel<KM>, dim3(p.G), dim3(256), 0, st, p);
+    return hipGetLastError();
+  }
+  const size_t lds = (size_t)(p.G + 1) * 4;
+  static LdsConfig cfg;
+  hipError_t e = ddrl_set_lds(snap_grad_first_kernel<KM>, lds, cfg);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(snap_grad_first_kernel<KM>, dim3(p.blocks + (p.n * p.k + 63) / 64), dim3(1024), lds, st, p, sort_bits(p.G));
+  return hipGetLastError();
+}
+extern "C" hipError_t snap_grad_launch(const SnapGrad *q, int pieces, hipStream_t st) {
+  SnapGrad p = *q;
+  p.piece = (p.blocks + pieces - 1) / pieces;
+  hipError_t e = p.k <= 2 ? grad_first_run<2>(p, st) : p.k <= 4 ? grad_first_run<4>(p, st) : grad_first_run<8>(p, st);
+  if (e != hipSuccess || !p.sorted) return e;
+  const dim3 grid(p.G, pieces);
+  if (p.S <= 64) hipLaunchKernelGGL(snap_grad_sum_kernel<1>, grid, dim3(256), 0, st, p);
+  else if (p.S <= 256) hipLaunchKernelGGL(snap_grad_sum_kernel<4>, grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL(snap_grad_sum_kernel<16>, grid, dim3(256), 0, st, p);
   return hipGetLastError();
 }

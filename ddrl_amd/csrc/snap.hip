@@ -29,7 +29,7 @@ struct DevBuf {                        // temporary device memory of a host-buff
 };
 bool off4(const void *p) { return ((uintptr_t)p & 3) != 0; }
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
-struct MixSpace { size_t count, idx, prob, y, ckey, cidx, all; int chunks; };
+struct MixSpace { size_t count, idx, prob, y, ckey, cidx, sorted, start, all; int chunks, blocks; };
 MixSpace mix_space(const ddrl_snap *s, int n, int k) {
   MixSpace w;
   const size_t places = (size_t)n * k;
@@ -41,12 +41,31 @@ MixSpace mix_space(const ddrl_snap *s, int n, int k) {
   w.chunks = snap_chunks(s->G, n, k);
   const size_t lists = w.chunks > 1 ? places * w.chunks : 0;
   w.cidx = w.ckey + up16(lists * 8);
-  w.all = w.cidx + up16(lists * 4);
+  w.sorted = w.cidx + up16(lists * 4);
+  w.blocks = places > SNAP_FEW ? snap_blocks(n, k) : 0;
+  w.start = w.sorted + (size_t)w.blocks * 1024 * 4;
+  w.all = w.start + up16((size_t)w.blocks * (s->G + 1) * 4);
+  return w;
+}
+struct GradSpace { size_t sorted, start, dlogit, done, sums, all; int blocks, pieces; };
+GradSpace grad_space(const ddrl_snap *s, int n, int k) {
+  GradSpace w;
+  const bool sort = (long long)n * k >= SNAP_SORT_FROM;
+  w.blocks = sort ? snap_blocks(n, k) : 0;
+  w.pieces = sort ? snap_grad_pieces(s->G, n, k) : 1;
+  w.sorted = 0;
+  w.start = (size_t)w.blocks * 1024 * 4;
+  w.dlogit = w.start + up16((size_t)w.blocks * (s->G + 1) * 4);
+  w.done = w.dlogit + (sort ? up16((size_t)n * k * 4) : 0);
+  w.sums = w.done + (w.pieces > 1 ? up16((size_t)s->G * 4) : 0);
+  w.all = w.sums + (w.pieces > 1 ? (size_t)w.pieces * s->G * (s->nd.lay[0].in + 1) * 8 : 0);
   return w;
 }
 int check_mix_shape(const ddrl_snap *s, int n, int k) {
   if (n < 0 || k < 1 || k > DDRL_SNAP_MAX_TOP_K || k > s->G)
     return ddrl_fail(DDRL_EINVAL, "n=%d, top_k=%d: n >= 0 and 1 <= top_k <= min(%d, %d agents)", n, k, DDRL_SNAP_MAX_TOP_K, s->G);
+  if ((int64_t)n * k >= SNAP_SORT_FROM / 4 && s->G > SNAP_SORT_MAX_G)
+    return ddrl_fail(DDRL_EINVAL, "n * top_k = %lld with %d agents: %d or more places are served for up to %d agents", (long long)n * k, s->G, SNAP_SORT_FROM / 4, SNAP_SORT_MAX_G);
   if ((int64_t)n * k > (1 << 28)) return ddrl_fail(DDRL_EINVAL, "n * top_k = %lld over %d", (long long)n * k, 1 << 28);
   return DDRL_OK;
 }
@@ -302,6 +321,7 @@ static int mixture_on(ddrl_snap *s, const ddrl_snap_mixture_args *a, hipStream_t
   p.prob = a->prob ? a->prob : (float *)(ws + w.prob);
   p.y = a->y ? a->y : (float *)(ws + w.y);
   p.ckey = (unsigned long long *)(ws + w.ckey); p.cidx = (int *)(ws + w.cidx); p.chunks = w.chunks;
+  p.sorted = (int *)(ws + w.sorted); p.start = (int *)(ws + w.start); p.blocks = w.blocks;
   HIPCHK(snap_mixture_launch(&s->nd, &p, st));
   return DDRL_OK;
 }
@@ -350,7 +370,7 @@ extern "C" int ddrl_snap_mixture(ddrl_snap_t *s, int n, int top_k, const float *
 extern "C" int ddrl_snap_mixture_grad_workspace(ddrl_snap_t *s, int n, int top_k, size_t *bytes) {
   if (!s || !bytes) return ddrl_fail(DDRL_EINVAL, "NULL argument");
   int rc = check_mix_shape(s, n, top_k);
-  if (!rc) *bytes = 0;
+  if (!rc) *bytes = grad_space(s, n, top_k).all;
   return rc;
 }
 
@@ -370,7 +390,18 @@ extern "C" int ddrl_snap_mixture_grad_dev(ddrl_snap_t *s, const ddrl_snap_mixtur
   p.db = a->d_router_b; p.dy = a->dy;
   if (p.x_row < 0 || p.dout_row < 0) return ddrl_fail(DDRL_EINVAL, "negative stride");
   if (p.dw_row < 0 || (p.G > 1 && p.dw_row < p.S)) return ddrl_fail(DDRL_EINVAL, "d_router_row=%lld: rows of d_router_w overlap", (long long)p.dw_row);
+  const GradSpace w = grad_space(s, a->n, a->top_k);
+  if (w.all && (!a->workspace || ((uintptr_t)a->workspace & 15) || a->workspace_bytes < w.all))
+    return ddrl_fail(DDRL_EINVAL, "workspace NULL, misaligned or under the %zu bytes of ddrl_snap_mixture_grad_workspace", w.all);
+  char *ws = (char *)a->workspace;
+  p.blocks = w.blocks;
+  p.sorted = w.blocks ? (int *)(ws + w.sorted) : nullptr;
+  p.start = w.blocks ? (int *)(ws + w.start) : nullptr;
+  p.dlogit = w.blocks ? (float *)(ws + w.dlogit) : nullptr;
+  p.done = (int *)(ws + w.done);
+  p.sums = w.pieces > 1 ? (double *)(ws + w.sums) : nullptr;
+  p.piece = 0;
   ON_DEVICE(s);
-  HIPCHK(snap_grad_launch(&p, (hipStream_t)a->stream));
+  HIPCHK(snap_grad_launch(&p, w.pieces, (hipStream_t)a->stream));
   return DDRL_OK;
 }

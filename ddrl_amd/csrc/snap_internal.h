@@ -76,6 +76,7 @@ struct SnapMixture {
   int *count;                         // [n] places of a row that are answered
   unsigned long long *ckey; int *cidx;   // [n x chunks x k] each chunk's best, where the router's agents are spread over several workgroups
   int chunks;
+  int *sorted, *start, blocks;        // idx sorted by net, a block of 1024 places at a time: [blocks x 1024], [blocks x (G + 1)]
 };
 struct SnapGrad {
   int G, n, k, S, A;
@@ -84,7 +85,21 @@ struct SnapGrad {
   const float *dout; int64_t dout_row;
   float *dw; int64_t dw_row;
   float *db, *dy;
+  int *sorted, *start, blocks;        // as in SnapMixture; null: few places, every workgroup looks through idx itself
+  float *dlogit;                      // [n x k]
+  double *sums;                       // [pieces x G x (S + 1)] where an agent's places are several workgroups' work
+  int *done;                          // [G] those that are through
+  int piece;                          // blocks of one of them
 };
+#define SNAP_SORT_FROM 1024            // places from which the gradient sorts them first
+#define SNAP_SORT_MAX_G 16383          // the sort keeps a counter a net in LDS
+static inline int snap_blocks(int n, int k) { return (int)(((long long)n * k + 1023) / 1024); }
+// how many workgroups an agent: a router prefers some agents, and the places of one are what a pass waits for
+static inline int snap_grad_pieces(int G, int n, int k) {
+  const int b = snap_blocks(n, k);
+  int p = (1024 + G - 1) / G;
+  return p > b ? (b < 1 ? 1 : b) : p;
+}
 
 // where the parameters of a load come from: the tile-major nets of a population, or flat rows
 struct SnapSource {
@@ -97,5 +112,5 @@ extern "C" {
 hipError_t snap_load_launch(const SnapDesc *nd, char *img, const SnapSource *src, int G, hipStream_t st);
 hipError_t snap_forward_launch(const SnapDesc *nd, const SnapForward *p, hipStream_t st);
 hipError_t snap_mixture_launch(const SnapDesc *nd, const SnapMixture *p, hipStream_t st);
-hipError_t snap_grad_launch(const SnapGrad *p, hipStream_t st);
+hipError_t snap_grad_launch(const SnapGrad *p, int pieces, hipStream_t st);
 }

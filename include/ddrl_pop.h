@@ -614,7 +614,8 @@ int ddrl_snap_forward(ddrl_snap_t *s, int n, const float *x, float *out);
  * among the allowed ones, the lower index first among equals (logits are summed in 64 bits, so that a pick does not hang on
  * the order of a sum; NaN counts as larger than any number, -infinity as not allowed), and
  *     prob[t, :] = softmax over the picked logits,   out[t] = sum_j prob[t, j] net_{idx[t, j]}(x[t]).
- * Where fewer than top_k are left, the last places of idx hold -1, of prob and y 0; a row with none has out = 0. */
+ * Where fewer than top_k are left, the last places of idx hold -1, of prob and y 0; a row with none has out = 0.
+ * n * top_k of 256 and more, here and in the gradient: up to 16383 agents. */
 typedef struct {
   int n, top_k;                            /* rows >= 0; 1 <= top_k <= min(DDRL_SNAP_MAX_TOP_K, n_agents) */
   const float *x; int64_t x_row;           /* [n x in_dim] */
