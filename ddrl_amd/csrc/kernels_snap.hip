@@ -11,7 +11,7 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // The kernels' first argument in the kernel-argument memory itself: a layer is one scalar load there, whatever its number
 // (a run-time index into the by-value argument would make the compiler copy it to scratch memory)
@@ -95,7 +95,7 @@ snap_load_kernel(const SnapDesc nd_, const SnapSource src, char *__restrict__ im
       unsigned c = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) c |= (none ? 0u : snap_code(v[i] * inv)) << (4 * i);
-      *(unsigned *)(rec + s * 256 + lane * 4) = c;
+      *(unsigned *)(rec + snap_code_off(steps, s, lane)) = c;
       if (q == 0) rec[snap_scale_off(y.code, s, r)] = (char)(none ? 127 : sh + 127);
     }
     if (q == 0) for (int s = steps; s & 3; ++s) rec[snap_scale_off(y.code, s, r)] = 127;
@@ -130,20 +130,29 @@ extern "C" hipError_t snap_load_launch(const SnapDesc *nd, char *img, const Snap
 // With 4 bits and R < 16 the columns 4 t, 4 t + 1, 4 t + 2 are the parts of row t: ONE product, summed over the columns at the
 // end.  And with R < 16 every lane finishes ONE output of the tile (bias, activation, the three parts) instead of a few lanes
 // finishing four: with few rows that, not the product, is most of the instructions.
+// Activations lie as the B operand is read, [k-step][part][16 rows][k quarter][row] x 16 bytes: a wave's read is 1 KiB without a
+// bank conflict, every one of a block of steps at a constant distance from the first.  Instructions, not bytes, bound a net
+// of many rows, so what is left of addresses is a scalar or such a constant.
 // ------------------------------------------------------------------------------------------------------------------------
-struct SnapLds { int second, image, first; };   // the inputs of layers 0, 2 lie in the first LDS buffer, those of 1, 3 in the second; behind them the image from byte `first` on, where it is staged
+struct SnapLds { int second, image; };          // the inputs of layers 0, 2 lie in the first LDS buffer, those of 1, 3 in the second; behind them the image, where it is staged
 
 template <int BITS, int R, int NT>
 struct SnapShape {
+  static_assert(BITS == 4 || R != 4, "four rows: 4 bits only");
   static constexpr int T = R * NT;                               // rows of a tile (NT > 1: R = 16)
-  static constexpr int ROWS = BITS == 4 ? 3 * T : T;             // rows of an LDS buffer: 4 bits: the rows' first parts, their second ones, their third
-  // a row's stride = 16 (mod 32) bytes, so that the 16 lanes that read 16 bytes of 16 rows at once start on distinct banks
-  __host__ __device__ static int ld(int K) { return BITS == 4 ? ddrl_roundup(K, 32) * 2 + 16 : ddrl_roundup(K, 16) * 4 + 16; }
+  static constexpr int P = BITS == 4 && R == 16 ? 3 : 1;         // products a step
+  static constexpr int COLS = R > 1 ? 16 : BITS == 4 ? 4 : 1;
+  static constexpr int QS = COLS * 16, TS = 4 * QS, XS = P * NT * TS;   // bytes from quarter to quarter, from tile of 16 rows (or part) to the next, from step to step
+  // part p of input k of row t
+  __device__ static __forceinline__ int at(int t, int p, int k) {
+    if (BITS == 4) return (k >> 5) * XS + (k >> 3 & 3) * QS + (k & 7) * 2 + (R == 16 ? (p * NT + (t >> 4)) * TS + (t & 15) * 16 : (4 * t + p) * 16);
+    return (k >> 4) * XS + (k >> 2 & 3) * QS + (k & 3) * 4 + (t >> 4) * TS + (t & 15) * 16;
+  }
   static int bytes(const SnapDesc &nd, SnapLds &m) {
     int a = 0, b = 0;
-    for (int l = 0; l < nd.L; ++l) { int &w = l & 1 ? b : a; w = ld(nd.lay[l].in) > w ? ld(nd.lay[l].in) : w; }
-    m.second = ROWS * a;
-    return m.image = ROWS * (a + b);
+    for (int l = 0; l < nd.L; ++l) { int &w = l & 1 ? b : a; w = nd.lay[l].steps * XS > w ? nd.lay[l].steps * XS : w; }
+    m.second = a;
+    return m.image = a + b;
   }
 };
 
@@ -168,7 +177,7 @@ __device__ __forceinline__ unsigned two_tops(float lo, float hi) { return __buil
 template <int BITS, int R, int NT, class Rows>
 __device__ __forceinline__ void tile_in(int K, char *buf, Rows rows) {
   using S = SnapShape<BITS, R, NT>;
-  const int ld = S::ld(K), Kp = BITS == 4 ? (K + 31) & ~31 : (K + 15) & ~15;
+  const int Kp = BITS == 4 ? (K + 31) & ~31 : (K + 15) & ~15;
   const int per = Kp <= 32 ? 32 : 64;                      // threads a row
 #pragma unroll 2
   for (int t = threadIdx.x / per; t < S::T; t += blockDim.x / per) {
@@ -181,8 +190,8 @@ __device__ __forceinline__ void tile_in(int K, char *buf, Rows rows) {
         float p[3];
         split3(v, p);
 #pragma unroll
-        for (int j = 0; j < 3; ++j) *(unsigned short *)(buf + (j * S::T + t) * ld + k * 2) = bf_top(p[j]);
-      } else *(float *)(buf + t * ld + k * 4) = v;
+        for (int j = 0; j < 3; ++j) *(unsigned short *)(buf + S::at(t, j, k)) = bf_top(p[j]);
+      } else *(float *)(buf + S::at(t, 0, k)) = v;
     }
   }
 }
@@ -198,64 +207,44 @@ __device__ __forceinline__ void lds_barrier() {
 template <int L>
 __device__ __forceinline__ float quad_lane(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), L * 0x55, 0xf, 0xf, true)); }
 
-// One k-step of MT strips.  `x`: the step's inputs of this lane's row
-template <int BITS, int R, int NT, int MT, class W>
-__device__ __forceinline__ void step_multiply(const W (&w)[MT], const unsigned (&sc)[MT], int byte, f32x4 (&acc)[MT][NT], const char *x, int ldi) {
-  if constexpr (BITS == 4) {
-    constexpr int P = R == 16 ? 3 : 1;
-    bf16x8 v[NT][P];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int p = 0; p < P; ++p) v[t][p] = *(const bf16x8 *)(x + (p * R * NT + 16 * t) * ldi);
-    union { bf16x2 h[4]; bf16x8 v; } a[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const float scale = __uint_as_float(((sc[i] >> byte) & 255u) << 23);
-      a[i].h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i], scale, 0);
-      a[i].h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i], scale, 1);
-      a[i].h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i], scale, 2);
-      a[i].h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[i], scale, 3);
-    }
-#pragma unroll
-    for (int p = P - 1; p >= 0; --p)                // the small parts first; products of one sum apart from each other
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i].v, v[t][p], acc[i][t], 0, 0, 0);
-  } else if constexpr (R == 1) {
-    const f32x4 v = *(const f32x4 *)x;
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][0][j] = fmaf(w[i][j], v[j], acc[i][0][j]);
-  } else {
-    f32x4 v[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) v[t] = *(const f32x4 *)(x + 16 * t * ldi);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i][j], v[t][j], acc[i][t], 0, 0, 0);
+// What a wave works on: strips s .. s + MT - 1 of layer l; where their records start in the image (of a strip that the layer does
+// not have: the last one's)
+struct Item { LayerOf y; int l, s; };
+template <int MT>
+__device__ __forceinline__ bool next_item(Item &it, DescP nd, int wave, int waves) {
+  it.s += waves * MT;
+  while (it.s >= it.y.strips) {
+    if (++it.l >= nd->L) return false;
+    it.y = layer_of(nd, it.l);
+    it.s = wave * MT;
   }
+  return true;
+}
+template <int MT>
+__device__ __forceinline__ void records(unsigned (&rec)[MT], const LayerOf &y, int s) {
+#pragma unroll
+  for (int i = 0; i < MT; ++i) rec[i] = y.off + (unsigned)min(s + i, y.strips - 1) * y.rec;
 }
 
-// UB k-steps of MT strips, asked for together; those beyond the layer's last step fetch that one again
-template <int BITS, int MT, int UB> struct SnapBlock {
-  using W = std::conditional_t<BITS == 4, unsigned, f32x4>;
-  W w[UB][MT];
-  unsigned sc[(UB + 3) / 4][MT];
-  __device__ __forceinline__ void load(const LayerOf &y, const char *const (&rec)[MT], int b, int lane) {
-    constexpr int SB = BITS == 4 ? 256 : 1024;               // bytes of a step
+// Four k-steps of MT strips, asked for together.  32 bits: those beyond the layer's last step are whatever follows in the image.
+template <int BITS, int MT> struct SnapBlock {
+  using W = std::conditional_t<BITS == 4, u32x4, f32x4[4]>;
+  W w[MT];
+  unsigned sc[MT];
+  template <bool LDS>
+  __device__ __forceinline__ void load(const char *img, const unsigned (&rec)[MT], const LayerOf &y, int b, unsigned lane) {
+    const bool whole = 4 * b + 4 <= y.steps;
+    const unsigned mine = whole ? lane * 16 : lane * (4 * (y.steps & 3));
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
+      if constexpr (BITS == 4) {
+        const char *from = img + (rec[i] + b * 1024u);
+        if (LDS && whole) w[i] = *(const u32x4 *)(from + mine);
+        else w[i] = *(const u32x4u *)(from + mine);
+        sc[i] = *(const unsigned *)(img + (rec[i] + y.code + b * 64u) + (lane & 15) * 4);
+      } else {
 #pragma unroll
-      for (int j = 0; j < UB; ++j) w[j][i] = *(const W *)(rec[i] + min(b + j, y.steps - 1) * SB + lane * sizeof(W));
-      if (BITS == 4) {
-#pragma unroll
-        for (int j = 0; j < UB; j += 4) sc[j / 4][i] = *(const unsigned *)(rec[i] + y.code + min(b + j, (y.steps - 1) & ~3) * 16 + (lane & 15) * 4);
+        for (int j = 0; j < 4; ++j) w[i][j] = *(const f32x4 *)(img + (rec[i] + b * 4096u) + lane * 16 + j * 1024);
       }
     }
   }
@@ -264,43 +253,69 @@ template <int BITS, int MT, int UB> struct SnapBlock {
   __device__ __forceinline__ void here() {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-#pragma unroll
-      for (int j = 0; j < UB; ++j) asm volatile("" : "+v"(w[j][i]));
-      if (BITS == 4) {
-#pragma unroll
-        for (int j = 0; j < UB; j += 4) asm volatile("" : "+v"(sc[j / 4][i]));
-      }
+      if constexpr (BITS == 4) { asm volatile("" : "+v"(w[i])); asm volatile("" : "+v"(sc[i])); }
+      else { _Pragma("unroll") for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(w[i][j])); }
     }
   }
 };
 
-// What a wave works on: strips s .. s + MT - 1 of layer l
-struct Item { LayerOf y; int l, s; };
-template <int MT>
-__device__ __forceinline__ bool next_item(Item &it, DescP nd, int end, int wave, int waves) {
-  it.s += waves * MT;
-  while (it.s >= it.y.strips) {
-    if (++it.l >= end) return false;
-    it.y = layer_of(nd, it.l);
-    it.s = wave * MT;
-  }
-  return true;
-}
-template <int MT>
-__device__ __forceinline__ void records(const char *(&rec)[MT], const Item &it, const char *img) {
+// Step j of a block.  `x`: the block's inputs of this lane's column
+template <int BITS, int R, int NT, int MT>
+__device__ __forceinline__ void step_multiply(const SnapBlock<BITS, MT> &w, int j, f32x4 (&acc)[MT][NT], const char *x) {
+  using S = SnapShape<BITS, R, NT>;
+  if constexpr (BITS == 4) {
+    bf16x8 v[NT][S::P];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) rec[i] = img + it.y.off + min(it.s + i, it.y.strips - 1) * it.y.rec;
+    for (int p = S::P - 1; p >= 0; --p)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) v[t][p] = *(const bf16x8 *)(x + j * S::XS + (p * NT + t) * S::TS);
+    union { bf16x2 h[4]; bf16x8 v; } a[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const float scale = __uint_as_float((w.sc[i] >> (8 * j) & 255u) << 23);
+      a[i].h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w.w[i][j], scale, 0);
+      a[i].h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w.w[i][j], scale, 1);
+      a[i].h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w.w[i][j], scale, 2);
+      a[i].h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w.w[i][j], scale, 3);
+    }
+#pragma unroll
+    for (int p = S::P - 1; p >= 0; --p)             // the small parts first; products of one sum apart from each other
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i].v, v[t][p], acc[i][t], 0, 0, 0);
+  } else if constexpr (R == 1) {
+    const f32x4 v = *(const f32x4 *)(x + j * S::XS);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[i][0][k] = fmaf(w.w[i][j][k], v[k], acc[i][0][k]);
+  } else {
+    f32x4 v[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) v[t] = *(const f32x4 *)(x + j * S::XS + t * S::TS);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w.w[i][j][k], v[t][k], acc[i][t], 0, 0, 0);
+  }
 }
+
 // The biases a lane needs.  R = 16: of its 4 outputs of every strip; R = 4: of the one of every strip; R = 1: of its one.
 template <int BITS, int R, int MT> struct SnapBias {
   f32x4 v4[R == 16 ? MT : 1];
   float v1[R == 4 ? MT : 1];
-  __device__ __forceinline__ void load(const Item &it, const char *const (&rec)[MT], const char *img, int c, int q) {
-    if constexpr (R == 16) { _Pragma("unroll") for (int i = 0; i < MT; ++i) v4[i] = *(const f32x4 *)(rec[i] + it.y.rec - 64 + q * 16); }
-    else if constexpr (R == 4) { _Pragma("unroll") for (int i = 0; i < MT; ++i) v1[i] = *(const float *)(rec[i] + it.y.rec - 64 + (4 * q + (c & 3)) * 4); }
+  __device__ __forceinline__ void load(const char *img, const unsigned (&rec)[MT], const LayerOf &y, unsigned c, unsigned q) {
+    const unsigned b = y.rec - 64;
+    if constexpr (R == 16) { _Pragma("unroll") for (int i = 0; i < MT; ++i) v4[i] = *(const f32x4 *)(img + (rec[i] + b) + q * 16); }
+    else if constexpr (R == 4) { _Pragma("unroll") for (int i = 0; i < MT; ++i) v1[i] = *(const float *)(img + (rec[i] + b) + (4 * q + (c & 3)) * 4); }
     else {
-      const int own = BITS == 4 ? (c >> 2) & (MT - 1) : q & (MT - 1), at = BITS == 4 ? 4 * q + (c & 3) : c;
-      v1[0] = *(const float *)(img + it.y.off + min(it.s + own, it.y.strips - 1) * it.y.rec + it.y.rec - 64 + at * 4);
+      const unsigned own = BITS == 4 ? (c >> 2) & (MT - 1) : q & (MT - 1), at = BITS == 4 ? 4 * q + (c & 3) : c;
+      unsigned from = rec[0];
+      _Pragma("unroll") for (int i = 1; i < MT; ++i) from = own == i ? rec[i] : from;
+      v1[0] = *(const float *)(img + (from + b + at * 4));
     }
   }
   __device__ __forceinline__ void here() {
@@ -309,39 +324,42 @@ template <int BITS, int R, int MT> struct SnapBias {
   }
 };
 // What is asked for before the inputs are there: the first block of a wave's first strips
-template <int BITS, int R, int MT, int UB> struct SnapAhead { Item it; bool any; SnapBlock<BITS, MT, UB> w; SnapBias<BITS, R, MT> bias; };
-template <int BITS, int R, int MT, int UB>
-__device__ __forceinline__ void ahead_load(SnapAhead<BITS, R, MT, UB> &h, const char *img, int lane) {
-  const char *rec[MT];
-  records<MT>(rec, h.it, img);
-  h.bias.load(h.it, rec, img, lane & 15, lane >> 4);
-  h.w.load(h.it.y, rec, 0, lane);
+template <int BITS, int R, int MT> struct SnapAhead { Item it; SnapBlock<BITS, MT> w; SnapBias<BITS, R, MT> bias; };
+template <int BITS, int R, int MT>
+__device__ __forceinline__ void ahead_load(SnapAhead<BITS, R, MT> &h, const char *img, unsigned lane) {
+  unsigned rec[MT];
+  records<MT>(rec, h.it.y, h.it.s);
+  h.bias.load(img, rec, h.it.y, lane & 15, lane >> 4);
+  h.w.template load<false>(img, rec, h.it.y, 0, lane);
 }
-template <int BITS, int R, int MT, int UB>
-__device__ __forceinline__ void ahead_first(SnapAhead<BITS, R, MT, UB> &h, DescP nd, const char *img, int end) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+template <int BITS, int R, int MT>
+__device__ __forceinline__ void ahead_first(SnapAhead<BITS, R, MT> &h, DescP nd, const char *img) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   h.it.y = layer_of(nd, 0); h.it.l = 0; h.it.s = (wave - waves) * MT;
-  h.any = next_item<MT>(h.it, nd, end, wave, waves);
-  if (h.any) ahead_load(h, img, lane);
+  if (next_item<MT>(h.it, nd, wave, waves)) ahead_load(h, img, threadIdx.x & 63);
 }
 
-// Layers from .. end - 1.  The inputs are in LDS, behind a barrier; `img`: the net's image, in memory (AHEAD: `h` comes from
+// All layers.  The inputs are in LDS, behind a barrier; `img`: the net's image, in memory (AHEAD: `h` comes from
 // ahead_first, and whatever is next, of the next layer too, is on its way while something is multiplied) or in LDS.  Ends with a
 // barrier.
-template <int BITS, int R, int NT, int MT, int UB, bool AHEAD, class Out>
-__device__ __forceinline__ void net_layers(SnapAhead<BITS, R, MT, UB> &h, DescP nd, const SnapLds &m, const char *img, char *lds, int from, int end_, Out out) {
+template <int BITS, int R, int NT, int MT, bool AHEAD, class Out>
+__device__ __forceinline__ void net_layers(SnapAhead<BITS, R, MT> &h, DescP nd, const SnapLds &m, const char *img, char *lds, Out out) {
   using S = SnapShape<BITS, R, NT>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, c = lane & 15, q = lane >> 4;
-  const int xrow = R == 16 ? c : (R == 4 ? c >> 2 : 0) + (BITS == 4 ? min(c & 3, 2) * S::T : 0);
-  LayerOf coming = layer_of(nd, from);
+  const int col = R == 16 ? c : BITS == 32 ? 0 : (R == 4 ? c & 12 : 0) + min(c & 3, 2);
+  // of the strip's outputs, this lane's (R = 16: its first): where it lies as an input of the next layer
+  const int at = R == 16 ? 4 * q : BITS == 4 ? 4 * q + (c & 3) : c;
+  const int put = R == 16 ? (BITS == 4 ? (q >> 1) * S::QS + (q & 1) * 8 : q * S::QS) + c * 16
+                  : BITS == 4 ? (at >> 3) * S::QS + (R == 4 ? c & 12 : 0) * 16 + (at & 7) * 2 : at * 4;
+  LayerOf coming = layer_of(nd, 0);
 #pragma unroll 1
-  for (int l = from; l < end_; ++l) {
+  for (int l = 0; l < nd->L; ++l) {
     const LayerOf y = coming;
     coming = layer_of(nd, min(l + 1, SNAP_MAXL - 1));
-    const int ldi = S::ld(y.in), ldo = S::ld(y.out);
-    const char *xin = lds + (l & 1 ? m.second : 0) + xrow * ldi + q * 16;
-    char *xout = lds + (l & 1 ? 0 : m.second);
+    const char *xin = lds + (l & 1 ? m.second : 0) + (q * S::QS + col * 16);
+    char *xout = lds + (l & 1 ? 0 : m.second) + put;
     const bool last = l == nd->L - 1;
+    const int blocks = (y.steps + 3) >> 2;
 #pragma unroll 1
     for (int s = wave * MT; s < y.strips; s += waves * MT) {
       f32x4 acc[MT][NT];
@@ -349,38 +367,35 @@ __device__ __forceinline__ void net_layers(SnapAhead<BITS, R, MT, UB> &h, DescP 
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const char *rec[MT];
+      unsigned rec[MT];
+      records<MT>(rec, y, s);
       SnapBias<BITS, R, MT> bias;
-      if (AHEAD) {
-        records<MT>(rec, h.it, img);
-        h.bias.here();
-        bias = h.bias;
-      } else {
-        const Item it = {y, l, s};
-        records<MT>(rec, it, img);
-        bias.load(it, rec, img, c, q);
-      }
+      if (AHEAD) { h.bias.here(); bias = h.bias; }
+      else bias.load(img, rec, y, c, q);
+      const char *x = xin;
 #pragma unroll 1
-      for (int b = 0; b < y.steps; b += UB) {
-        SnapBlock<BITS, MT, UB> next;
+      for (int b = 0; b < blocks; ++b) {
+        SnapBlock<BITS, MT> next;
         if (AHEAD) {
           h.w.here();
-          if (b + UB < y.steps) next.load(y, rec, b + UB, lane);
-        } else h.w.load(y, rec, b, lane);
-        if (b + UB <= y.steps) {
+          if (b + 1 < blocks) next.template load<false>(img, rec, y, b + 1, lane);
+        } else h.w.template load<true>(img, rec, y, b, lane);
+        const int now = y.steps - 4 * b;
+        if (now >= 4) {
 #pragma unroll
-          for (int j = 0; j < UB; ++j) step_multiply<BITS, R, NT, MT>(h.w.w[j], h.w.sc[j / 4], 8 * (j & 3), acc, xin + (b + j) * 64, ldi);
+          for (int j = 0; j < 4; ++j) step_multiply<BITS, R, NT, MT>(h.w, j, acc, x);
         } else {
 #pragma unroll
-          for (int j = 0; j < UB - 1; ++j)
-            if (j == 0 || b + j < y.steps) step_multiply<BITS, R, NT, MT>(h.w.w[j], h.w.sc[j / 4], 8 * (j & 3), acc, xin + (b + j) * 64, ldi);
+          for (int j = 0; j < 3; ++j)
+            if (j == 0 || j < now) step_multiply<BITS, R, NT, MT>(h.w, j, acc, x);
         }
+        x += 4 * S::XS;
         if (AHEAD) h.w = next;
       }
-      if (AHEAD && next_item<MT>(h.it, nd, end_, wave, waves)) ahead_load(h, img, lane);
+      if (AHEAD && next_item<MT>(h.it, nd, wave, waves)) ahead_load(h, img, lane);
       const bool odd = BITS == 4 && (y.strips & 1);            // the next layer's k-steps are 32 wide: zeros behind an odd last strip
       if constexpr (R < 16) {
-        const int own = R > 1 ? 0 : BITS == 4 ? (c >> 2) & (MT - 1) : q & (MT - 1), at = BITS == 4 || R == 4 ? 4 * q + (c & 3) : c;
+        const int own = R > 1 ? 0 : BITS == 4 ? (c >> 2) & (MT - 1) : q & (MT - 1);
 #pragma unroll
         for (int i = 0; i < (R == 1 ? 1 : MT); ++i) {
           float v;
@@ -406,10 +421,8 @@ __device__ __forceinline__ void net_layers(SnapAhead<BITS, R, MT, UB> &h, DescP 
                 for (int j = 0; j < 4; ++j) p[j] = own == k ? acc[k][0][j] : p[j];
               strip = s + own;
             }
-            if constexpr (BITS == 4) {                         // the parts lie in the lanes of a quad: smallest first
 #pragma unroll
-              for (int j = 0; j < 4; ++j) p[j] = quad_lane<0>((quad_lane<2>(p[j]) + quad_lane<1>(p[j])) + p[j]);
-            }
+            for (int j = 0; j < 4; ++j) p[j] = quad_lane<0>((quad_lane<2>(p[j]) + quad_lane<1>(p[j])) + p[j]);   // the parts lie in the lanes of a quad: smallest first
             const int j = c & 3;
             v = j & 1 ? p[1] : p[0];
             const float v2 = j & 1 ? p[3] : p[2];
@@ -424,21 +437,22 @@ __device__ __forceinline__ void net_layers(SnapAhead<BITS, R, MT, UB> &h, DescP 
             else if constexpr (BITS == 4) {
               float p[3];
               split3(v, p);
+              char *o = xout + strip * (2 * S::QS);
 #pragma unroll
               for (int k = 0; k < 3; ++k) {
-                char *o = xout + (k * S::T + t) * ldo + n * 2;
-                *(unsigned short *)o = bf_top(p[k]);
-                if (odd && strip == y.strips - 1) *(unsigned short *)(o + 32) = 0;
+                *(unsigned short *)(o + k * 16) = bf_top(p[k]);
+                if (odd && strip == y.strips - 1) *(unsigned short *)(o + 2 * S::QS + k * 16) = 0;
               }
-            } else *(float *)(xout + t * ldo + n * 4) = v;
+            } else *(float *)(xout + strip * S::XS) = v;
           }
         }
       } else {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
           if (s + i < y.strips) {
-            const int n0 = (s + i) * 16 + 4 * q;
-            const bool end = s + i == y.strips - 1;
+            const int strip = s + i, n0 = strip * 16 + 4 * q;
+            const bool end = strip == y.strips - 1;
+            char *o = xout + (BITS == 4 ? (strip >> 1) * S::XS + (strip & 1) * (2 * S::QS) : strip * S::XS);
 #pragma unroll
             for (int tt = 0; tt < NT; ++tt) {
               const int t = 16 * tt + c;
@@ -458,15 +472,14 @@ __device__ __forceinline__ void net_layers(SnapAhead<BITS, R, MT, UB> &h, DescP 
                   for (int j = 0; j < 4; ++j) r[j] = r[j] != r[j] ? 0.f : r[j];
                 }
                 const f32x4 lo = rest4(r);
-                char *o = xout + t * ldo + n0 * 2;
-                *(u32x2 *)o = u32x2{two_tops(a[0], a[1]), two_tops(a[2], a[3])};
-                *(u32x2 *)(o + S::T * ldo) = u32x2{two_tops(r[0], r[1]), two_tops(r[2], r[3])};
-                *(u32x2 *)(o + 2 * S::T * ldo) = u32x2{two_tops(lo[0], lo[1]), two_tops(lo[2], lo[3])};
+                *(u32x2 *)(o + tt * S::TS) = u32x2{two_tops(a[0], a[1]), two_tops(a[2], a[3])};
+                *(u32x2 *)(o + (NT + tt) * S::TS) = u32x2{two_tops(r[0], r[1]), two_tops(r[2], r[3])};
+                *(u32x2 *)(o + (2 * NT + tt) * S::TS) = u32x2{two_tops(lo[0], lo[1]), two_tops(lo[2], lo[3])};
                 if (odd && end) {
 #pragma unroll
-                  for (int k = 0; k < 3; ++k) *(u32x2 *)(o + k * S::T * ldo + 32) = u32x2{0u, 0u};
+                  for (int k = 0; k < 3; ++k) *(u32x2 *)(o + (k * NT + tt) * S::TS + 2 * S::QS) = u32x2{0u, 0u};
                 }
-              } else *(f32x4 *)(xout + t * ldo + n0 * 4) = a;
+              } else *(f32x4 *)(o + tt * S::TS) = a;
             }
           }
       }
@@ -485,37 +498,36 @@ __device__ __forceinline__ void image_in(const char *img, char *lds, unsigned by
 }
 __device__ __forceinline__ void image_here() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// How a workgroup comes by its net: straight from memory as it goes (0), all of it staged in LDS (1), or all but the first layer
-// (2), which goes to registers meanwhile.  net_ask before the inputs are brought in, net_tile after them.
-template <int BITS, int R, int NT, int MT, int UB, int STAGE> struct SnapNet {
-  SnapAhead<BITS, R, MT, UB> h;
+// How a workgroup comes by its net: straight from memory as it goes, or all of it staged in LDS.  net_ask before the inputs are
+// brought in, net_tile after them.
+template <int BITS, int R, int NT, int MT, bool STAGED> struct SnapNet {
+  SnapAhead<BITS, R, MT> h;
   const char *img;
   __device__ __forceinline__ void stage(DescP nd, const SnapLds &m, const char *image, char *lds) {      // once for a net
     img = image;
-    if (STAGE) image_in(image + m.first, lds + m.image, nd->stride - m.first);
+    if (STAGED) image_in(image, lds + m.image, nd->stride);
   }
-  __device__ __forceinline__ void ask(DescP nd) { if (STAGE != 1) ahead_first(h, nd, img, STAGE ? 1 : nd->L); }     // for a tile
+  __device__ __forceinline__ void ask(DescP nd) { if (!STAGED) ahead_first(h, nd, img); }     // for a tile
   template <class Out>
   __device__ __forceinline__ void tile(DescP nd, const SnapLds &m, char *lds, Out out) {
-    if (STAGE) image_here();
+    if (STAGED) image_here();
     lds_barrier();
-    if (STAGE != 1) net_layers<BITS, R, NT, MT, UB, true>(h, nd, m, img, lds, 0, STAGE ? 1 : nd->L, out);
-    if (STAGE) net_layers<BITS, R, NT, MT, UB, false>(h, nd, m, lds + (m.image - m.first), lds, STAGE - 1, nd->L, out);
+    net_layers<BITS, R, NT, MT, !STAGED>(h, nd, m, STAGED ? lds + m.image : img, lds, out);
   }
 };
 
 // ------------------------------------------------------------------------------------------------------------------------
 // Every agent's net on its rows
 // ------------------------------------------------------------------------------------------------------------------------
-template <int BITS, int R, int NT, int MT, int UB, int STAGE>
-__global__ void __launch_bounds__(R == 16 && STAGE == 2 ? 1024 : 512)
+template <int BITS, int R, int NT, int MT, bool STAGED>
+__global__ void __launch_bounds__(R == 16 && !STAGED ? 1024 : 512)
 snap_forward_kernel(const SnapDesc nd_, const SnapLds m, const SnapForward p) {
   extern __shared__ __align__(16) char lds[];
   using S = SnapShape<BITS, R, NT>;
   const DescP nd = SNAP_DESC(nd_);
   const int g = blockIdx.x;
   if (p.mask && !p.mask[g]) return;
-  SnapNet<BITS, R, NT, MT, UB, STAGE> net;
+  SnapNet<BITS, R, NT, MT, STAGED> net;
   net.stage(nd, m, p.img + (size_t)g * nd->stride, lds);
   const int from = blockIdx.y * p.per, to = min(p.n, from + p.per);
 #pragma unroll 1
@@ -721,7 +733,7 @@ snap_router_kernel(const SnapMixture p, int S, int A, int ld) {
 // answered in.  The answers are stored past the XCD's own cache (agent scope); once they have arrived the counter may tell of
 // them.  Nothing else passes between workgroups, so no cache has to be written back or forgotten, and nobody waits.
 // ------------------------------------------------------------------------------------------------------------------------
-template <int BITS, int MT, int UB, int STAGE>
+template <int BITS, int MT, bool STAGED>
 __global__ void __launch_bounds__(512)
 snap_place_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
   extern __shared__ __align__(16) char lds[];
@@ -749,7 +761,7 @@ snap_place_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
     }
   }
   if (e < 0) return;
-  SnapNet<BITS, 1, 1, MT, UB, STAGE> net;
+  SnapNet<BITS, 1, 1, MT, STAGED> net;
   net.stage(nd, m, p.img + (size_t)e * nd->stride, lds);
   net.ask(nd);
   const float *x = p.x + row * p.x_row;
@@ -861,7 +873,7 @@ __device__ __forceinline__ int place_of(const Segments &g, const int *sorted, in
 // The picked nets, many places: a workgroup answers, for one net, every gridDim.y-th tile of T of the places that picked it; the
 // rows are summed up as above.
 // ------------------------------------------------------------------------------------------------------------------------
-template <int BITS, int R, int NT, int MT, int UB, int STAGE>
+template <int BITS, int R, int NT, int MT, bool STAGED>
 __global__ void __launch_bounds__(512)
 snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
   extern __shared__ __align__(16) char lds[];
@@ -870,7 +882,7 @@ snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
   __shared__ int list[S::T], done[S::T];
   const DescP nd = SNAP_DESC(nd_);
   const int tid = threadIdx.x, A = nd->A, threads = blockDim.x, e = blockIdx.x;
-  SnapNet<BITS, R, NT, MT, UB, STAGE> net;
+  SnapNet<BITS, R, NT, MT, STAGED> net;
   bool staged = false;
   for (int b0 = 0; b0 < p.blocks; b0 += 256) {
     const int have = segments_of(seg, p.start, p.n * p.k, p.G, e, b0, min(256, p.blocks - b0));
@@ -1116,56 +1128,53 @@ static int waves_for(const SnapDesc &nd, int mt, int most) {
   return waves > most ? most : waves;
 }
 // the LDS of a kernel, and where in it what lies
-template <int BITS, int R, int NT, int STAGE>
-static int lds_for(const SnapDesc &nd, SnapLds &m) {
-  const int x = SnapShape<BITS, R, NT>::bytes(nd, m);
-  m.first = STAGE == 2 ? nd.lay[1].off & ~1023 : 0;
-  return x + (STAGE ? nd.stride - m.first : 0);
-}
-template <int BITS, int R, int NT, int STAGE>
-static bool fits(const SnapDesc &nd, int most) { SnapLds m; return lds_for<BITS, R, NT, STAGE>(nd, m) <= most; }
+template <int BITS, int R, int NT, bool STAGED>
+static int lds_for(const SnapDesc &nd, SnapLds &m) { return SnapShape<BITS, R, NT>::bytes(nd, m) + (STAGED ? nd.stride + (BITS == 32 ? SNAP_OVER : 0) : 0); }
+template <int BITS, int R, int NT, bool STAGED>
+static bool fits(const SnapDesc &nd, int most) { SnapLds m; return lds_for<BITS, R, NT, STAGED>(nd, m) <= most; }
 
-template <int BITS, int R, int NT, int MT, int UB, int STAGE>
-static hipError_t forward_run(const SnapDesc &nd, SnapForward p, int most_waves, hipStream_t st) {
+#define SNAP_HALF (SNAP_LDS / 2)      // two workgroups a CU: one computes while the other's net arrives
+template <int BITS, int R, int MT, bool STAGED>
+static hipError_t forward_run(const SnapDesc &nd, SnapForward p, hipStream_t st) {
   SnapLds m;
-  const int lds = lds_for<BITS, R, NT, STAGE>(nd, m), T = R * NT;
+  const int lds = lds_for<BITS, R, 1, STAGED>(nd, m);
   static LdsConfig cfg;
-  const auto kernel = snap_forward_kernel<BITS, R, NT, MT, UB, STAGE>;
+  const auto kernel = snap_forward_kernel<BITS, R, 1, MT, STAGED>;
   hipError_t e = ddrl_set_lds(kernel, lds, cfg);
   if (e != hipSuccess) return e;
-  const int tiles = (p.n + T - 1) / T;
-  int chunks = p.G >= 1024 ? 1 : (1024 + p.G - 1) / p.G;
+  const int tiles = (p.n + R - 1) / R;
+  // 2048 workgroups where there are as many tiles (129 agents, 24-100-100-1, 250 rows: 17 us, with 1024 21 us)
+  int chunks = (2048 + p.G - 1) / p.G;
   if (chunks > tiles) chunks = tiles;
   const int per = (tiles + chunks - 1) / chunks;
-  p.per = per * T;
-  hipLaunchKernelGGL(kernel, dim3(p.G, (tiles + per - 1) / per), dim3(waves_for(nd, MT, most_waves) * 64), lds, st, nd, m, p);
+  p.per = per * R;
+  // 8 waves, so that two workgroups share a CU and one computes at the other's barriers; where the activations leave room for
+  // one only, 16 (1024 agents, 64 rows: 18-400-300-6 with 8 waves 105 us, with 16 132 us; 18-600-500-6 275 and 219 us)
+  const int most = R == 16 && !STAGED && lds > SNAP_HALF ? 16 : 8;
+  hipLaunchKernelGGL(kernel, dim3(p.G, (tiles + per - 1) / per), dim3(waves_for(nd, MT, most) * 64), lds, st, nd, m, p);
   return hipGetLastError();
 }
 
-#define SNAP_HALF (SNAP_LDS / 2)      // two workgroups a CU: one computes while the other's net arrives
+// Rows a tile: n of 2 to 4 as 4 (4 bits; 1024 agents of 18-400-300-6, 4 rows: 23 us, in tiles of 16 28 us), more as 16.
+// Staged or not: a net that lets two workgroups share a CU is staged whole (1024 agents, 18-100-100-6: 16 rows 9.6 us, unstaged
+// 12.5; 1 row 7.3 and 7.7).  A larger one goes from memory to registers (18-400-300-6, all but its first layer staged: 1 row 27
+// us, unstaged 22; 64 rows 147 and 105).
+// Strips a wave: two share a read of the inputs but leave waves idle; with very few strips, or more than the 8 waves, one (64
+// rows: 18-20-20-6 two 13.7 us, one 12.0; 24-200-200-1 67 and 57; 250 rows of 18-100-100-6: 8.7 and 10.3).
 extern "C" hipError_t snap_forward_launch(const SnapDesc *nd, const SnapForward *p, hipStream_t st) {
-  const bool deep = nd->L > 1;
   if (nd->bits == 4) {
     if (p->n > 4) {
-      if (fits<4, 16, 1, 1>(*nd, SNAP_HALF)) return forward_run<4, 16, 1, 2, 4, 1>(*nd, *p, 8, st);
-      if (deep && fits<4, 16, 1, 2>(*nd, SNAP_LDS)) return forward_run<4, 16, 1, 2, 4, 2>(*nd, *p, 16, st);
-      if (fits<4, 16, 1, 0>(*nd, SNAP_LDS)) return forward_run<4, 16, 1, 4, 4, 0>(*nd, *p, 8, st);
+      if (fits<4, 16, 1, true>(*nd, SNAP_HALF)) {
+        const int strips = most_strips(*nd);
+        return strips > 2 && strips <= 8 ? forward_run<4, 16, 2, true>(*nd, *p, st) : forward_run<4, 16, 1, true>(*nd, *p, st);
+      }
+      if (fits<4, 16, 1, false>(*nd, SNAP_LDS)) return forward_run<4, 16, 1, false>(*nd, *p, st);
     }
-    if (p->n > 1) {
-      if (fits<4, 4, 1, 1>(*nd, SNAP_HALF)) return forward_run<4, 4, 1, 2, 4, 1>(*nd, *p, 8, st);
-      if (deep && fits<4, 4, 1, 2>(*nd, SNAP_HALF)) return forward_run<4, 4, 1, 2, 4, 2>(*nd, *p, 8, st);
-      return forward_run<4, 4, 1, 2, 4, 0>(*nd, *p, 8, st);
-    }
-    if (fits<4, 1, 1, 1>(*nd, SNAP_HALF)) return forward_run<4, 1, 1, 2, 4, 1>(*nd, *p, 8, st);
-    if (deep && fits<4, 1, 1, 2>(*nd, SNAP_HALF)) return forward_run<4, 1, 1, 2, 4, 2>(*nd, *p, 8, st);
-    return forward_run<4, 1, 1, 2, 4, 0>(*nd, *p, 8, st);
+    if (p->n > 1) return fits<4, 4, 1, true>(*nd, SNAP_HALF) ? forward_run<4, 4, 2, true>(*nd, *p, st) : forward_run<4, 4, 1, false>(*nd, *p, st);
+    return fits<4, 1, 1, true>(*nd, SNAP_HALF) ? forward_run<4, 1, 2, true>(*nd, *p, st) : forward_run<4, 1, 2, false>(*nd, *p, st);
   }
-  if (p->n > 1) {
-    if (fits<32, 16, 1, 1>(*nd, SNAP_HALF)) return forward_run<32, 16, 1, 2, 4, 1>(*nd, *p, 8, st);
-    return forward_run<32, 16, 1, 2, 4, 0>(*nd, *p, 8, st);
-  }
-  if (fits<32, 1, 1, 1>(*nd, SNAP_HALF)) return forward_run<32, 1, 1, 2, 4, 1>(*nd, *p, 8, st);
-  return forward_run<32, 1, 1, 2, 4, 0>(*nd, *p, 8, st);
+  if (p->n > 1) return fits<32, 16, 1, true>(*nd, SNAP_HALF) ? forward_run<32, 16, 2, true>(*nd, *p, st) : forward_run<32, 16, 1, false>(*nd, *p, st);
+  return fits<32, 1, 1, true>(*nd, SNAP_HALF) ? forward_run<32, 1, 2, true>(*nd, *p, st) : forward_run<32, 1, 2, false>(*nd, *p, st);
 }
 
 template <int KM>
@@ -1181,23 +1190,23 @@ static hipError_t router_run(const SnapMixture &p, int S, int A, hipStream_t st)
   hipLaunchKernelGGL(snap_router_kernel<KM>, dim3((p.n + 15) / 16, p.chunks), dim3(waves * 64), lds, st, p, S, A, ld);
   return hipGetLastError();
 }
-template <int BITS, int MT, int UB, int STAGE>
+template <int BITS, int MT, bool STAGED>
 static hipError_t place_run(const SnapDesc &nd, const SnapMixture &p, hipStream_t st) {
   SnapLds m;
-  const int lds = lds_for<BITS, 1, 1, STAGE>(nd, m);
+  const int lds = lds_for<BITS, 1, 1, STAGED>(nd, m);
   static LdsConfig cfg;
-  const auto kernel = snap_place_kernel<BITS, MT, UB, STAGE>;
+  const auto kernel = snap_place_kernel<BITS, MT, STAGED>;
   hipError_t e = ddrl_set_lds(kernel, lds, cfg);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kernel, dim3(p.n * p.k), dim3(waves_for(nd, MT, 8) * 64), lds, st, nd, m, p);
   return hipGetLastError();
 }
-template <int BITS, int R, int NT, int MT, int UB, int STAGE>
+template <int BITS, int R, int NT, int MT, bool STAGED>
 static hipError_t experts_run(const SnapDesc &nd, const SnapMixture &p, hipStream_t st) {
   SnapLds m;
-  const int lds = lds_for<BITS, R, NT, STAGE>(nd, m);
+  const int lds = lds_for<BITS, R, NT, STAGED>(nd, m);
   static LdsConfig cfg;
-  const auto kernel = snap_experts_kernel<BITS, R, NT, MT, UB, STAGE>;
+  const auto kernel = snap_experts_kernel<BITS, R, NT, MT, STAGED>;
   hipError_t e = ddrl_set_lds(kernel, lds, cfg);
   if (e != hipSuccess) return e;
   int waves = waves_for(nd, MT, 8);
@@ -1233,22 +1242,19 @@ extern "C" hipError_t snap_mixture_launch(const SnapDesc *nd, const SnapMixture 
                                                                                                               : router_run<8>(*p, S, A, st);
   if (e != hipSuccess) return e;
   const int total = p->n * p->k, left = SNAP_LDS - SNAP_STATIC_LDS;
-  const bool deep = nd->L > 1;
   if (total <= SNAP_FEW) {
-    if (nd->bits == 4)
-      return fits<4, 1, 1, 1>(*nd, SNAP_HALF) ? place_run<4, 2, 4, 1>(*nd, *p, st)
-             : deep && fits<4, 1, 1, 2>(*nd, SNAP_LDS - 1024) ? place_run<4, 2, 4, 2>(*nd, *p, st) : place_run<4, 2, 4, 0>(*nd, *p, st);
-    return fits<32, 1, 1, 1>(*nd, SNAP_HALF) ? place_run<32, 2, 4, 1>(*nd, *p, st) : place_run<32, 2, 4, 0>(*nd, *p, st);
+    if (nd->bits == 4) return fits<4, 1, 1, true>(*nd, SNAP_HALF) ? place_run<4, 2, true>(*nd, *p, st) : place_run<4, 2, false>(*nd, *p, st);
+    return fits<32, 1, 1, true>(*nd, SNAP_HALF) ? place_run<32, 2, true>(*nd, *p, st) : place_run<32, 2, false>(*nd, *p, st);
   }
   if ((e = sort_run(p->idx, total, p->G, p->sorted, p->start, st)) != hipSuccess) return e;
   if (nd->bits == 4) {
-    if (fits<4, 16, 1, 1>(*nd, left)) return experts_run<4, 16, 1, 2, 4, 1>(*nd, *p, st);
-    if (fits<4, 16, 1, 0>(*nd, left)) return experts_run<4, 16, 1, 4, 4, 0>(*nd, *p, st);
-    return experts_run<4, 4, 1, 2, 4, 0>(*nd, *p, st);
+    if (fits<4, 16, 1, true>(*nd, left)) return experts_run<4, 16, 1, 2, true>(*nd, *p, st);
+    if (fits<4, 16, 1, false>(*nd, left)) return experts_run<4, 16, 1, 1, false>(*nd, *p, st);
+    return experts_run<4, 4, 1, 1, false>(*nd, *p, st);
   }
-  if (fits<32, 16, 1, 1>(*nd, left)) return experts_run<32, 16, 1, 1, 4, 1>(*nd, *p, st);
-  if (fits<32, 16, 1, 0>(*nd, left)) return experts_run<32, 16, 1, 1, 4, 0>(*nd, *p, st);
-  return experts_run<32, 1, 1, 2, 4, 0>(*nd, *p, st);
+  if (fits<32, 16, 1, true>(*nd, left)) return experts_run<32, 16, 1, 1, true>(*nd, *p, st);
+  if (fits<32, 16, 1, false>(*nd, left)) return experts_run<32, 16, 1, 1, false>(*nd, *p, st);
+  return experts_run<32, 1, 1, 2, false>(*nd, *p, st);
 }
 
 template <int KM>

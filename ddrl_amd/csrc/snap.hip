@@ -109,7 +109,7 @@ extern "C" int ddrl_snap_create(int n_agents, int in_dim, int out_dim, const int
   if (!s) return ddrl_fail(DDRL_ENOMEM, "out of host memory");
   s->G = n_agents; s->device = device;
   snap_build_desc(s->nd, in_dim, hidden, n_hidden, out_dim, hidden_layer_type, output_layer_type, bits);
-  const size_t bytes = (size_t)n_agents * s->nd.stride;
+  const size_t bytes = (size_t)n_agents * s->nd.stride + SNAP_OVER;
   auto bail = [&](int code, const char *what, hipError_t e) {
     const int rc = ddrl_fail(code, "%s: %s", what, hipGetErrorString(e));
     ddrl_snap_destroy(s);
@@ -222,7 +222,7 @@ extern "C" int ddrl_snap_get_weights(ddrl_snap_t *s, double *flat) {
               const int r = o & 15;
               if (n.bits == 4) {
                 unsigned c;
-                memcpy(&c, rec + (k >> 5) * 256 + (((k >> 3) & 3) * 16 + r) * 4, 4);
+                memcpy(&c, rec + snap_code_off(y.steps, k >> 5, ((k >> 3) & 3) * 16 + r), 4);
                 const unsigned char e = (unsigned char)rec[snap_scale_off(y.code, k >> 5, r)];
                 *f++ = std::ldexp(grid[(c >> (4 * (k & 7))) & 15], (int)e - 127);
               } else {

@@ -16,7 +16,8 @@
 // contiguous piece of memory in lane order (lane = 16 q + r <-> output r of the strip):
 //   32 bits: a k-step is 16 inputs, lane (r, q) holds inputs 4q .. 4q+3 as one float4: 1 KiB a step;
 //    4 bits: a k-step is 32 inputs, lane (r, q) holds inputs 8q .. 8q+7 as one dword of codes (lowest input in the lowest
-//            bits): 256 bytes a step.  Behind the steps the scales, a byte each (E8M0: 2^(byte - 127)), [step / 4][output][step % 4].
+//            bits): 256 bytes a step.  Four steps lie together, [lane][step], 16 bytes a lane; the last steps % 4 too, with as
+//            many dwords a lane.  Behind the steps the scales, a byte each (E8M0: 2^(byte - 127)), [step / 4][output][step % 4].
 // A record ends with the 16 biases, fp32.  Outputs are padded to strips and inputs to k-steps with zeros.
 struct SnapLayer {
   int in, out, strips, steps;
@@ -46,6 +47,12 @@ static inline void snap_build_desc(SnapDesc &n, int d0, const int *hidden, int n
   }
   n.stride = (off + 1023) / 1024 * 1024;
 }
+// where the codes of (step, lane) lie in a record
+__host__ __device__ inline unsigned snap_code_off(int steps, int step, int lane) {
+  const int whole = steps & ~3, in4 = step < whole ? 4 : steps & 3;
+  return (step & ~3) * 256 + lane * 4 * in4 + (step & 3) * 4;
+}
+#define SNAP_OVER 4096         // bytes behind the last image that a 32-bit kernel may read (never use): whatever it asks for, it asks for four steps
 // where the scale of (output r of a strip, step) lies in a record
 __host__ __device__ inline unsigned snap_scale_off(int code, int step, int r) { return (unsigned)code + (step >> 2) * 64 + r * 4 + (step & 3); }
 
