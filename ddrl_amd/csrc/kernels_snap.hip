@@ -173,17 +173,21 @@ __device__ __forceinline__ f32x4 rest4(f32x4 x) {
 }
 __device__ __forceinline__ unsigned two_tops(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
 
-// `rows(t)`: where row t of the tile lies, or null; all threads of the workgroup, no barrier inside
+// The waves that answer a tile together: a whole workgroup, or one of several equal parts of it
+struct Team { int tid, threads, wave, waves; };
+__device__ __forceinline__ Team whole_team() { return {(int)threadIdx.x, (int)blockDim.x, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), (int)(blockDim.x >> 6)}; }
+
+// `rows(t)`: where row t of the tile lies, or null; all threads of the team, no barrier inside
 template <int BITS, int R, int NT, class Rows>
-__device__ __forceinline__ void tile_in(int K, char *buf, Rows rows) {
+__device__ __forceinline__ void tile_in(const Team &w, int K, char *buf, Rows rows) {
   using S = SnapShape<BITS, R, NT>;
   const int Kp = BITS == 4 ? (K + 31) & ~31 : (K + 15) & ~15;
   const int per = Kp <= 32 ? 32 : 64;                      // threads a row
 #pragma unroll 2
-  for (int t = threadIdx.x / per; t < S::T; t += blockDim.x / per) {
+  for (int t = w.tid / per; t < S::T; t += w.threads / per) {
     const float *x = rows(t);
 #pragma unroll 1
-    for (int k = threadIdx.x & (per - 1); k < Kp; k += per) {
+    for (int k = w.tid & (per - 1); k < Kp; k += per) {
       float v = x && k < K ? x[k] : 0.f;
       if (BITS == 4) {
         v = v != v ? __uint_as_float(0x7fc00000u) : v;     // (a NaN that its upper half alone would not show)
@@ -333,25 +337,25 @@ __device__ __forceinline__ void ahead_load(SnapAhead<BITS, R, MT> &h, const char
   h.w.template load<false>(img, rec, h.it.y, 0, lane);
 }
 template <int BITS, int R, int MT>
-__device__ __forceinline__ void ahead_first(SnapAhead<BITS, R, MT> &h, DescP nd, const char *img) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  h.it.y = layer_of(nd, 0); h.it.l = 0; h.it.s = (wave - waves) * MT;
-  if (next_item<MT>(h.it, nd, wave, waves)) ahead_load(h, img, threadIdx.x & 63);
+__device__ __forceinline__ void ahead_first(const Team &w, SnapAhead<BITS, R, MT> &h, DescP nd, const char *img) {
+  h.it.y = layer_of(nd, 0); h.it.l = 0; h.it.s = (w.wave - w.waves) * MT;
+  if (next_item<MT>(h.it, nd, w.wave, w.waves)) ahead_load(h, img, threadIdx.x & 63);
 }
 
 // All layers.  The inputs are in LDS, behind a barrier; `img`: the net's image, in memory (AHEAD: `h` comes from
 // ahead_first, and whatever is next, of the next layer too, is on its way while something is multiplied) or in LDS.  Ends with a
 // barrier.
 template <int BITS, int R, int NT, int MT, bool AHEAD, class Out>
-__device__ __forceinline__ void net_layers(SnapAhead<BITS, R, MT> &h, DescP nd, const SnapLds &m, const char *img, char *lds, Out out) {
+__device__ __forceinline__ void net_layers(const Team &w, SnapAhead<BITS, R, MT> &h, DescP nd, const SnapLds &m, const char *img, char *lds, Out out) {
   using S = SnapShape<BITS, R, NT>;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, c = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = w.wave, waves = w.waves, c = lane & 15, q = lane >> 4;
   const int col = R == 16 ? c : BITS == 32 ? 0 : (R == 4 ? c & 12 : 0) + min(c & 3, 2);
   // of the strip's outputs, this lane's (R = 16: its first): where it lies as an input of the next layer
   const int at = R == 16 ? 4 * q : BITS == 4 ? 4 * q + (c & 3) : c;
   const int put = R == 16 ? (BITS == 4 ? (q >> 1) * S::QS + (q & 1) * 8 : q * S::QS) + c * 16
                   : BITS == 4 ? (at >> 3) * S::QS + (R == 4 ? c & 12 : 0) * 16 + (at & 7) * 2 : at * 4;
   LayerOf coming = layer_of(nd, 0);
+  asm volatile("" : "+s"(coming.steps));                       // (here: a wait inside the loop would be one for the next layer's too)
 #pragma unroll 1
   for (int l = 0; l < nd->L; ++l) {
     const LayerOf y = coming;
@@ -489,10 +493,10 @@ __device__ __forceinline__ void net_layers(SnapAhead<BITS, R, MT> &h, DescP nd, 
 }
 
 // A net's image from memory to LDS, without a register in between: everything is asked for at once.  The caller waits.
-__device__ __forceinline__ void image_in(const char *img, char *lds, unsigned bytes) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+__device__ __forceinline__ void image_in(const Team &w, const char *img, char *lds, unsigned bytes) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll 1
-  for (unsigned i = wave * 1024; i < bytes; i += waves * 1024)
+  for (unsigned i = w.wave * 1024; i < bytes; i += w.waves * 1024)
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(img + i + lane * 16),
                                      (__attribute__((address_space(3))) void *)(lds + i), 16, 0, 0);
 }
@@ -503,16 +507,18 @@ __device__ __forceinline__ void image_here() { asm volatile("s_waitcnt vmcnt(0)"
 template <int BITS, int R, int NT, int MT, bool STAGED> struct SnapNet {
   SnapAhead<BITS, R, MT> h;
   const char *img;
+  Team w;
+  __device__ __forceinline__ SnapNet(const Team &team) : w(team) {}
   __device__ __forceinline__ void stage(DescP nd, const SnapLds &m, const char *image, char *lds) {      // once for a net
     img = image;
-    if (STAGED) image_in(image, lds + m.image, nd->stride);
+    if (STAGED) image_in(w, image, lds + m.image, nd->stride);
   }
-  __device__ __forceinline__ void ask(DescP nd) { if (!STAGED) ahead_first(h, nd, img); }     // for a tile
+  __device__ __forceinline__ void ask(DescP nd) { if (!STAGED) ahead_first(w, h, nd, img); }     // for a tile
   template <class Out>
   __device__ __forceinline__ void tile(DescP nd, const SnapLds &m, char *lds, Out out) {
     if (STAGED) image_here();
     lds_barrier();
-    net_layers<BITS, R, NT, MT, !STAGED>(h, nd, m, STAGED ? lds + m.image : img, lds, out);
+    net_layers<BITS, R, NT, MT, !STAGED>(w, h, nd, m, STAGED ? lds + m.image : img, lds, out);
   }
 };
 
@@ -527,14 +533,14 @@ snap_forward_kernel(const SnapDesc nd_, const SnapLds m, const SnapForward p) {
   const DescP nd = SNAP_DESC(nd_);
   const int g = blockIdx.x;
   if (p.mask && !p.mask[g]) return;
-  SnapNet<BITS, R, NT, MT, STAGED> net;
+  SnapNet<BITS, R, NT, MT, STAGED> net(whole_team());
   net.stage(nd, m, p.img + (size_t)g * nd->stride, lds);
   const int from = blockIdx.y * p.per, to = min(p.n, from + p.per);
 #pragma unroll 1
   for (int t0 = from; t0 < to; t0 += S::T) {
     net.ask(nd);
     const float *x = p.x + g * p.x_agent + t0 * p.x_row;
-    tile_in<BITS, R, NT>(nd->lay[0].in, lds, [&](int t) { return t0 + t < to ? x + t * p.x_row : (const float *)nullptr; });
+    tile_in<BITS, R, NT>(net.w, nd->lay[0].in, lds, [&](int t) { return t0 + t < to ? x + t * p.x_row : (const float *)nullptr; });
     float *o = p.out + g * p.out_agent + t0 * p.out_row;
     net.tile(nd, m, lds, [&](int t, int n, float v) { if (t0 + t < to) o[t * p.out_row + n] = v; });
   }
@@ -571,34 +577,120 @@ __device__ __forceinline__ void best_dpp(unsigned long long &k, int &i) {
 __device__ __forceinline__ void best_of_16(unsigned long long &k, int &i) {
   best_dpp<0xB1>(k, i); best_dpp<0x4E>(k, i); best_dpp<0x141>(k, i); best_dpp<0x140>(k, i);
 }
+// Between the rows of 16: v_permlane16_swap(a, b) is {a's even rows, b's even rows in the odd places} and the same of the odd ones,
+// v_permlane32_swap the halves likewise
+struct Two { unsigned x, y; };
+template <bool HALVES>
+__device__ __forceinline__ Two swap_rows(unsigned a, unsigned b) {
+  const auto v = HALVES ? __builtin_amdgcn_permlane32_swap(a, b, false, false) : __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  return {v[0], v[1]};
+}
+template <bool HALVES>
+__device__ __forceinline__ void best_swap(unsigned long long &k, int &i) {
+  const Two h = swap_rows<HALVES>((unsigned)(k >> 32), (unsigned)(k >> 32)), l = swap_rows<HALVES>((unsigned)k, (unsigned)k), n = swap_rows<HALVES>((unsigned)i, (unsigned)i);
+  const unsigned long long ka = (unsigned long long)h.x << 32 | l.x, kb = (unsigned long long)h.y << 32 | l.y;
+  const bool a = key_before(ka, (int)n.x, kb, (int)n.y);
+  k = a ? ka : kb; i = (int)(a ? n.x : n.y);
+}
+// the sums over the two rows (halves) of a in the even ones, of b in the odd ones
+template <bool HALVES>
+__device__ __forceinline__ double sum_swap(double a, double b) {
+  const unsigned long long u = (unsigned long long)__double_as_longlong(a), v = (unsigned long long)__double_as_longlong(b);
+  const Two h = swap_rows<HALVES>((unsigned)(u >> 32), (unsigned)(v >> 32)), l = swap_rows<HALVES>((unsigned)u, (unsigned)v);
+  return __longlong_as_double((long long)((unsigned long long)h.x << 32 | l.x)) + __longlong_as_double((long long)((unsigned long long)h.y << 32 | l.y));
+}
+template <int CTRL>
+__device__ __forceinline__ unsigned long long most_dpp(unsigned long long k) {
+  const unsigned long long o = (unsigned long long)(unsigned)__builtin_amdgcn_update_dpp(0, (int)(k >> 32), CTRL, 0xf, 0xf, true) << 32 |
+                               (unsigned)__builtin_amdgcn_update_dpp(0, (int)k, CTRL, 0xf, 0xf, true);
+  return o > k ? o : k;
+}
+template <bool HALVES>
+__device__ __forceinline__ unsigned long long most_swap(unsigned long long k) {
+  const Two h = swap_rows<HALVES>((unsigned)(k >> 32), (unsigned)(k >> 32)), l = swap_rows<HALVES>((unsigned)k, (unsigned)k);
+  const unsigned long long ka = (unsigned long long)h.x << 32 | l.x, kb = (unsigned long long)h.y << 32 | l.y;
+  return ka > kb ? ka : kb;
+}
+// the largest of 64, as a scalar
+__device__ __forceinline__ unsigned long long most_of_64(unsigned long long k) {
+  k = most_dpp<0x140>(most_dpp<0x141>(most_dpp<0x4E>(most_dpp<0xB1>(k))));
+  k = most_swap<true>(most_swap<false>(k));
+  return (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(k >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)k);
+}
 #define IDX_NONE 0x7fffffff
-__device__ __forceinline__ int lane_of_16(int v, int j) { return __shfl(v, j, 16); }
+// the first of a row of 16's, in all of them
+__device__ __forceinline__ int first_of_16(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x150, 0xf, 0xf, true); }
+__device__ __forceinline__ float sum_of_16(float v) {
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, true));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, true));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, true));
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xf, 0xf, true));
+  return v;
+}
 
-// A row's picks from sorted lists of k: lane u of 16 looks at list u (lists <= 16), lane j keeps the j-th pick: its index (or
-// IDX_NONE) and, after the softmax, its probability
-template <class Key, class Idx>
-__device__ __forceinline__ void merge_16(int u, int lists, int k, Key key, Idx idx, int &mi, float &mp) {
-  int head = 0;
-  unsigned long long mk = KEY_NONE, nk = KEY_NONE;
-  int ni = IDX_NONE;
-  mi = IDX_NONE;
-  if (u < lists) { nk = key(0); ni = idx(0); }
-  for (int j = 0; j < k; ++j) {
-    unsigned long long bk = nk;
-    int bi = ni;
-    best_of_16(bk, bi);
-    if (bi != IDX_NONE && ni == bi) {
-      ++head;
-      const bool more = head < k;
-      nk = more ? key(head) : KEY_NONE; ni = more ? idx(head) : IDX_NONE;
-    }
-    if (u == j) { mk = bk; mi = bi; }
+// A lane's KM best, sorted
+template <int KM> struct Best {
+  unsigned long long K[KM];
+  int I[KM];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < KM; ++j) { K[j] = KEY_NONE; I[j] = IDX_NONE; }
   }
-  const double l = key_logit(mk), top = __shfl(l, 0, 16);
-  const float ex = mi != IDX_NONE ? expf((float)(l - top)) : 0.f;
-  float sum = 0.f;
-  for (int j = 0; j < k; ++j) sum += __shfl(ex, j, 16);
-  mp = mi != IDX_NONE ? ex / sum : 0.f;
+  __device__ __forceinline__ void insert(unsigned long long key, int e) {     // (after all of a lower index)
+    if (key > K[KM - 1]) {
+#pragma unroll
+      for (int i = 0; i < KM; ++i) {
+        const bool up = key > K[i];
+        const unsigned long long tk = K[i]; const int te = I[i];
+        K[i] = up ? key : tk; I[i] = up ? e : te;
+        key = up ? tk : key; e = up ? te : e;
+      }
+    }
+  }
+  __device__ __forceinline__ void pop(int i) {                                 // if i is the first
+    if (I[0] == i) {
+#pragma unroll
+      for (int j = 0; j + 1 < KM; ++j) { K[j] = K[j + 1]; I[j] = I[j + 1]; }
+      K[KM - 1] = KEY_NONE; I[KM - 1] = IDX_NONE;
+    }
+  }
+  // a list that lies in memory
+  template <class Key, class Idx> __device__ __forceinline__ void read(int k, Key key, Idx idx) {
+#pragma unroll
+    for (int j = 0; j < KM; ++j) if (j < k) { K[j] = key(j); I[j] = idx(j); }
+  }
+  // the k best of 16 lanes' lists: lane j keeps the j-th
+  __device__ __forceinline__ void merge_16(int lane, int k, unsigned long long &mk, int &mi) {
+    mk = KEY_NONE; mi = IDX_NONE;
+#pragma unroll 1
+    for (int j = 0; j < k; ++j) {
+      unsigned long long bk = K[0];
+      int bi = I[0];
+      best_of_16(bk, bi);
+      pop(bi);
+      if (lane == j) { mk = bk; mi = bi; }
+    }
+  }
+  // of 64: the largest key, then who has it, the lowest index among several (several: rare)
+  __device__ __forceinline__ void merge_64(int lane, int k, unsigned long long &mk, int &mi) {
+    mk = KEY_NONE; mi = IDX_NONE;
+#pragma unroll 1
+    for (int j = 0; j < k; ++j) {
+      const unsigned long long bk = most_of_64(K[0]);
+      if (bk == KEY_NONE) break;
+      int bi = IDX_NONE;
+      for (unsigned long long who = __ballot(K[0] == bk); who; who &= who - 1) bi = min(bi, __builtin_amdgcn_readlane(I[0], __ffsll(who) - 1));
+      pop(bi);
+      if (lane == j) { mk = bk; mi = bi; }
+    }
+  }
+};
+// the softmax over the picks that 16 lanes hold
+__device__ __forceinline__ float pick_prob(unsigned long long mk, int mi) {
+  const unsigned long long tk = (unsigned long long)(unsigned)first_of_16((int)(mk >> 32)) << 32 | (unsigned)first_of_16((int)mk);
+  const float ex = mi != IDX_NONE ? expf((float)(key_logit(mk) - key_logit(tk))) : 0.f;
+  const float sum = sum_of_16(ex);
+  return mi != IDX_NONE ? ex / sum : 0.f;
 }
 
 // grid (rows / 16, chunks): the rows' best among the agents [chunk * G / chunks, ..); with one chunk the picks themselves
@@ -615,10 +707,8 @@ snap_router_kernel(const SnapMixture p, int S, int A, int ld) {
   const int Sp = (S + 15) & ~15;
   for (int t = threadIdx.x >> 5; t < 16; t += blockDim.x >> 5)
     for (int k = threadIdx.x & 31; k < Sp; k += 32) xs[t * ld + k] = t0 + t < p.n && k < S ? p.x[(t0 + t) * p.x_row + k] : 0.f;
-  unsigned long long K[KM];
-  int I[KM];
-#pragma unroll
-  for (int j = 0; j < KM; ++j) { K[j] = KEY_NONE; I[j] = IDX_NONE; }
+  Best<KM> best;
+  best.clear();
   const int row = min(t0 + c, p.n - 1);
   const uint8_t *al = p.allowed ? p.allowed + row * p.a_row : nullptr;
   bool first = true;
@@ -658,35 +748,16 @@ snap_router_kernel(const SnapMixture p, int S, int A, int ld) {
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      int e = s * 16 + 4 * j + q;
-      unsigned long long key = ok[j] ? logit_key(acc[j] + (double)bias[j]) : KEY_NONE;
-      if (key > K[KM - 1]) {
-#pragma unroll
-        for (int i = 0; i < KM; ++i) {
-          const bool up = key > K[i];
-          const unsigned long long tk = K[i]; const int te = I[i];
-          K[i] = up ? key : tk; I[i] = up ? e : te;
-          key = up ? tk : key; e = up ? te : e;
-        }
-      }
+      best.insert(ok[j] ? logit_key(acc[j] + (double)bias[j]) : KEY_NONE, s * 16 + 4 * j + q);
     }
   }
   if (first) __syncthreads();
   // the four lanes of a row
   for (int j = 0; j < p.k; ++j) {
-    unsigned long long bk = K[0];
-    int bi = I[0];
-#pragma unroll
-    for (int d = 16; d <= 32; d *= 2) {
-      const unsigned long long ok = __shfl_xor(bk, d);
-      const int oi = __shfl_xor(bi, d);
-      if (key_before(ok, oi, bk, bi)) { bk = ok; bi = oi; }
-    }
-    if (I[0] == bi) {
-#pragma unroll
-      for (int i = 0; i + 1 < KM; ++i) { K[i] = K[i + 1]; I[i] = I[i + 1]; }
-      K[KM - 1] = KEY_NONE; I[KM - 1] = IDX_NONE;
-    }
+    unsigned long long bk = best.K[0];
+    int bi = best.I[0];
+    best_swap<false>(bk, bi); best_swap<true>(bk, bi);
+    best.pop(bi);
     if (q == 0) { ck[(c * waves + wave) * KM + j] = bk; ci[(c * waves + wave) * KM + j] = bi; }
   }
   __syncthreads();
@@ -694,63 +765,192 @@ snap_router_kernel(const SnapMixture p, int S, int A, int ld) {
   const int u = threadIdx.x & 15;
   for (int t = threadIdx.x >> 4; t < 16; t += blockDim.x >> 4) {
     const int tok = t0 + t;
-    const unsigned long long *lk = ck + (t * waves + (u < waves ? u : 0)) * KM;
-    const int *li = ci + (t * waves + (u < waves ? u : 0)) * KM;
+    const bool live = tok < p.n;
+    unsigned long long mk;
+    int mi;
+    best.clear();
+    if (u < waves) best.read(p.k, [&](int j) { return ck[(t * waves + u) * KM + j]; }, [&](int j) { return ci[(t * waves + u) * KM + j]; });
+    best.merge_16(u, p.k, mk, mi);
+    if (live && u == 0 && blockIdx.y == 0) p.count[tok] = 0;
     if (p.chunks > 1) {                                    // the chunk's list, sorted
-      int head = 0;
-      for (int j = 0; j < p.k; ++j) {
-        unsigned long long bk = KEY_NONE;
-        int bi = IDX_NONE;
-        if (u < waves && head < p.k) { bk = lk[head]; bi = li[head]; }
-        const int own = bi;
-        best_of_16(bk, bi);
-        if (own == bi && bi != IDX_NONE) ++head;
-        if (tok < p.n && u == j) {
-          p.ckey[((int64_t)tok * p.chunks + blockIdx.y) * p.k + j] = bk;
-          p.cidx[((int64_t)tok * p.chunks + blockIdx.y) * p.k + j] = bi;
-        }
+      if (live && u < p.k) {
+        p.ckey[((int64_t)tok * p.chunks + blockIdx.y) * p.k + u] = mk;
+        p.cidx[((int64_t)tok * p.chunks + blockIdx.y) * p.k + u] = mi;
       }
-      if (tok < p.n && u == 0 && blockIdx.y == 0) p.count[tok] = 0;
       continue;
     }
-    int mi;
-    float mp;
-    merge_16(u, waves, p.k, [&](int h) { return lk[h]; }, [&](int h) { return li[h]; }, mi, mp);
-    const bool have = mi != IDX_NONE, live = tok < p.n;
+    const float mp = pick_prob(mk, mi);
+    const bool have = mi != IDX_NONE;
     if (live && u < p.k) {
       p.idx[(int64_t)tok * p.k + u] = have ? mi : -1;
       p.prob[(int64_t)tok * p.k + u] = mp;
       if (!have) for (int a = 0; a < A; ++a) p.y[((int64_t)tok * p.k + u) * A + a] = 0.f;
     }
-    if (live && lane_of_16(mi, 0) == IDX_NONE) for (int a = u; a < A; a += 16) p.out[tok * p.out_row + a] = 0.f;
-    if (live && u == 0) p.count[tok] = 0;
+    if (live && first_of_16(mi) == IDX_NONE) for (int a = u; a < A; a += 16) p.out[tok * p.out_row + a] = 0.f;
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
-// The picked nets, few places: a workgroup for each.  It makes the row's picks out of the router's lists (or reads them), answers
-// its place, and whoever answers a row's last place sums the row up, in the order of its places whatever the order they were
-// answered in.  The answers are stored past the XCD's own cache (agent scope); once they have arrived the counter may tell of
-// them.  Nothing else passes between workgroups, so no cache has to be written back or forgotten, and nobody waits.
+// A row's picks, for a workgroup of its own: out of the router's lists, or read.  All threads; ends with a barrier.
+// ------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void row_picks(const SnapMixture &p, int row, int *picks, float *probs) {
+  const int tid = threadIdx.x;
+  if (p.chunks > 1) {
+    if (tid < 16) {
+      unsigned long long mk;
+      int mi;
+      const int64_t at = ((int64_t)row * p.chunks + tid) * p.k;
+      Best<SNAP_MAXK> best;
+      best.clear();
+      if (tid < p.chunks) best.read(p.k, [&](int j) { return p.ckey[at + j]; }, [&](int j) { return p.cidx[at + j]; });
+      best.merge_16(tid, p.k, mk, mi);
+      const float mp = pick_prob(mk, mi);
+      if (tid < p.k) { picks[tid] = mi == IDX_NONE ? -1 : mi; probs[tid] = mp; }
+    }
+  } else if (tid < p.k) { picks[tid] = p.idx[row * p.k + tid]; probs[tid] = p.prob[row * p.k + tid]; }
+  __syncthreads();
+}
+
+// ------------------------------------------------------------------------------------------------------------------------
+// Few rows, nets that fit in LDS together: a workgroup a row, a team of its waves for each pick, so that the answers meet in LDS.
+// And as long as the router's matrix is small, every workgroup works the router out for its row by itself (KM > 0), a thread an
+// agent at a time, sums in fp64 as above: one launch, nothing to hand over.  Bound by the latency of what follows on what: the
+// router's rows, the picks, the nets' images, the layers.
+// ------------------------------------------------------------------------------------------------------------------------
+// inputs at .. at + 3 of a router row of S, zeros behind its end; no lane reads beyond it
+__device__ __forceinline__ f32x4 row_four(const float *w, int at, int S) {
+  if (S < 4) return f32x4{at < S ? w[min(at, S - 1)] : 0.f, at + 1 < S ? w[min(at + 1, S - 1)] : 0.f, at + 2 < S ? w[min(at + 2, S - 1)] : 0.f, 0.f};
+  const f32x4 v = *(const f32x4u *)(w + min(at, S - 4));
+  const int d = at - (S - 4);
+  f32x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    r[j] = d <= 0 ? v[j] : 0.f;
+#pragma unroll
+    for (int i = 1; j + i < 4; ++i) r[j] = d == i ? v[j + i] : r[j];
+  }
+  return r;
+}
+// xs: the row's inputs, zeros behind them up to a multiple of 16.  A wave takes 64 agents at a time, as 4 times 16 whose rows are
+// read by 4 lanes each, 16 bytes a lane (a lane an agent would touch 64 lines with every read).
+template <int KM>
+__device__ __forceinline__ void route_row(const SnapMixture &p, int S, int row, const float *xs, char *lists, int *picks, float *probs) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6, c = lane & 15, q = lane >> 4;
+  unsigned long long *ck = (unsigned long long *)lists;     // [waves][KM]
+  int *ci = (int *)(ck + waves * KM);
+  Best<KM> best;
+  best.clear();
+  const uint8_t *al = p.allowed ? p.allowed + row * p.a_row : nullptr;
+  bool first = true;
+#pragma unroll 1
+  for (int e0 = wave * 64; e0 < p.G || first; e0 += waves * 64) {
+    const int e = min(e0 + lane, p.G - 1);
+    const float bias = p.rb ? p.rb[e] : 0.f;
+    const bool ok = e0 + lane < p.G && (!al || al[e]);
+    const float *w[4];
+    double acc[4] = {0., 0., 0., 0.};
+#pragma unroll
+    for (int m = 0; m < 4; ++m) w[m] = p.rw + (int64_t)min(e0 + 16 * m + c, p.G - 1) * p.r_row;
+#pragma unroll 1
+    for (int s0 = 0; s0 < S; s0 += 32) {
+      f32x4 a[4][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int at = s0 + 16 * u + 4 * q;
+        if (s0 + 16 * u + 16 <= S) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m) a[m][u] = *(const f32x4u *)(w[m] + at);
+        } else if (s0 + 16 * u < S) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m) a[m][u] = row_four(w[m], at, S);
+        }
+      }
+      if (first) { __syncthreads(); first = false; }        // (the inputs have come)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (s0 + 16 * u < S) {
+          const f32x4 x = *(const f32x4 *)(xs + s0 + 16 * u + 4 * q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) acc[m] = fma((double)a[m][u][j], (double)x[j], acc[m]);
+        }
+    }
+    const double sum = sum_swap<false>(sum_swap<true>(acc[0], acc[2]), sum_swap<true>(acc[1], acc[3]));   // lane 16 m + c: agent e0 + 16 m + c's
+    best.insert(ok ? logit_key(sum + (double)bias) : KEY_NONE, e);
+  }
+  unsigned long long mk;
+  int mi;
+  best.merge_64(lane, p.k, mk, mi);
+  if (p.G > 64) {
+    if (lane < p.k) { ck[wave * KM + lane] = mk; ci[wave * KM + lane] = mi; }
+    __syncthreads();
+    if (wave == 0) {
+      best.clear();
+      if (lane < waves) best.read(p.k, [&](int j) { return ck[lane * KM + j]; }, [&](int j) { return ci[lane * KM + j]; });
+      best.merge_64(lane, p.k, mk, mi);
+    }
+  }
+  if (wave == 0) {
+    const float mp = pick_prob(mk, mi);
+    if (lane < p.k) { picks[lane] = mi == IDX_NONE ? -1 : mi; probs[lane] = mp; }
+  }
+  __syncthreads();
+}
+// where what lies in the LDS of snap_row_kernel: the row's inputs, the waves' lists, the answers, a team's part
+struct SnapRow { int lists, y, teams, team, waves; };
+
+template <int BITS, int MT, int KM>
+__global__ void __launch_bounds__(1024)
+snap_row_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p, const SnapRow at) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ int picks[SNAP_MAXK];
+  __shared__ float probs[SNAP_MAXK];
+  const DescP nd = SNAP_DESC(nd_);
+  const int tid = threadIdx.x, A = nd->A, S = nd->lay[0].in, row = blockIdx.x;
+  float *xs = (float *)lds, *y = (float *)(lds + at.y);
+  const float *x = p.x + row * p.x_row;
+  for (int s = tid; s < ((S + 15) & ~15); s += blockDim.x) xs[s] = s < S ? x[s] : 0.f;
+  if (KM) route_row<KM ? KM : 1>(p, S, row, xs, lds + at.lists, picks, probs);
+  else row_picks(p, row, picks, probs);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = wave / at.waves;
+  const int e = j < p.k ? __builtin_amdgcn_readfirstlane(picks[j]) : -1;
+  // (who has no net keeps the barriers only: no strip is its own)
+  const Team w = {tid - j * at.waves * 64, at.waves * 64, e >= 0 ? wave - j * at.waves : SNAP_MAXW, at.waves};
+  char *own = lds + at.teams + (e >= 0 ? j : 0) * at.team;
+  SnapNet<BITS, 1, 1, MT, true> net(w);
+  if (e >= 0) {
+    net.stage(nd, m, p.img + (size_t)e * nd->stride, own);
+    tile_in<BITS, 1, 1>(w, S, own, [&](int) { return xs; });
+  }
+  if (tid < p.k && (KM || p.chunks > 1)) { p.idx[row * p.k + tid] = picks[tid]; p.prob[row * p.k + tid] = probs[tid]; }
+  net.tile(nd, m, own, [&](int, int n, float v) { y[j * A + n] = v; });
+  for (int a = tid; a < A; a += blockDim.x) {
+    float sum = 0.f;
+    for (int i = 0; i < p.k; ++i) {
+      const float v = picks[i] >= 0 ? y[i * A + a] : 0.f;
+      p.y[((int64_t)row * p.k + i) * A + a] = v;
+      sum = picks[i] >= 0 ? fmaf(probs[i], v, sum) : sum;
+    }
+    p.out[row * p.out_row + a] = sum;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------
+// Few places of larger nets: a workgroup for each.  Whoever answers a row's last place sums the row up, in the order of its places
+// whatever the order they were answered in.  The answers are stored past the XCD's own cache (agent scope); once they have arrived
+// the counter may tell of them.  Nothing else passes between workgroups, so no cache has to be written back or forgotten, and
+// nobody waits.
 // ------------------------------------------------------------------------------------------------------------------------
 template <int BITS, int MT, bool STAGED>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(STAGED ? 512 : 1024)
 snap_place_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
   extern __shared__ __align__(16) char lds[];
   __shared__ int picks[SNAP_MAXK], last;
   __shared__ float probs[SNAP_MAXK];
   const DescP nd = SNAP_DESC(nd_);
   const int tid = threadIdx.x, A = nd->A, row = blockIdx.x / p.k, place = blockIdx.x - row * p.k;
-  if (p.chunks > 1) {
-    if (tid < 16) {
-      int mi;
-      float mp;
-      const int64_t at = ((int64_t)row * p.chunks + (tid < p.chunks ? tid : 0)) * p.k;
-      merge_16(tid, p.chunks, p.k, [&](int h) { return p.ckey[at + h]; }, [&](int h) { return p.cidx[at + h]; }, mi, mp);
-      if (tid < p.k) { picks[tid] = mi == IDX_NONE ? -1 : mi; probs[tid] = mp; }
-    }
-  } else if (tid < p.k) { picks[tid] = p.idx[row * p.k + tid]; probs[tid] = p.prob[row * p.k + tid]; }
-  __syncthreads();
+  row_picks(p, row, picks, probs);
   const int e = __builtin_amdgcn_readfirstlane(picks[place]);
   float *y = p.y + (int64_t)blockIdx.x * A;
   if (p.chunks > 1) {
@@ -761,11 +961,11 @@ snap_place_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
     }
   }
   if (e < 0) return;
-  SnapNet<BITS, 1, 1, MT, STAGED> net;
+  SnapNet<BITS, 1, 1, MT, STAGED> net(whole_team());
   net.stage(nd, m, p.img + (size_t)e * nd->stride, lds);
   net.ask(nd);
   const float *x = p.x + row * p.x_row;
-  tile_in<BITS, 1, 1>(nd->lay[0].in, lds, [&](int) { return x; });
+  tile_in<BITS, 1, 1>(net.w, nd->lay[0].in, lds, [&](int) { return x; });
   net.tile(nd, m, lds, [&](int, int n, float v) { __hip_atomic_store(y + n, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
@@ -882,7 +1082,7 @@ snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
   __shared__ int list[S::T], done[S::T];
   const DescP nd = SNAP_DESC(nd_);
   const int tid = threadIdx.x, A = nd->A, threads = blockDim.x, e = blockIdx.x;
-  SnapNet<BITS, R, NT, MT, STAGED> net;
+  SnapNet<BITS, R, NT, MT, STAGED> net(whole_team());
   bool staged = false;
   for (int b0 = 0; b0 < p.blocks; b0 += 256) {
     const int have = segments_of(seg, p.start, p.n * p.k, p.G, e, b0, min(256, p.blocks - b0));
@@ -891,7 +1091,7 @@ snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
       net.ask(nd);
       if (tid < S::T) list[tid] = i0 + tid < have ? place_of(seg, p.sorted, i0 + tid) : -1;
       __syncthreads();
-      tile_in<BITS, R, NT>(nd->lay[0].in, lds, [&](int t) { return list[t] >= 0 ? p.x + (int64_t)(list[t] / p.k) * p.x_row : (const float *)nullptr; });
+      tile_in<BITS, R, NT>(net.w, nd->lay[0].in, lds, [&](int t) { return list[t] >= 0 ? p.x + (int64_t)(list[t] / p.k) * p.x_row : (const float *)nullptr; });
       net.tile(nd, m, lds, [&](int t, int n, float v) {
         if (list[t] >= 0) __hip_atomic_store(p.y + (int64_t)list[t] * A + n, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       });
@@ -931,13 +1131,6 @@ snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
 // workgroups each, a run of sorted blocks every one; their sums go to the workspace, and the last of them adds all, in order.
 // Sums over rows are in fp64 (an agent may be picked by every row).
 // ------------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float sum_of_16(float v) {
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, true));
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, true));
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, true));
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xf, 0xf, true));
-  return v;
-}
 // dlogit of a place, in all of its 16 lanes (a0 = 0 .. 15), and dy; one that picked nobody: 0
 template <int KM>
 __device__ __forceinline__ float dlogit_of(const SnapGrad &p, int place, int a0) {
@@ -1190,6 +1383,28 @@ static hipError_t router_run(const SnapMixture &p, int S, int A, hipStream_t st)
   hipLaunchKernelGGL(snap_router_kernel<KM>, dim3((p.n + 15) / 16, p.chunks), dim3(waves * 64), lds, st, p, S, A, ld);
   return hipGetLastError();
 }
+template <int BITS, int KM>
+static hipError_t row_run(const SnapDesc &nd, const SnapMixture &p, const SnapLds &m, SnapRow at, int lds, hipStream_t st) {
+  static LdsConfig cfg;
+  const auto kernel = snap_row_kernel<BITS, 2, KM>;
+  hipError_t e = ddrl_set_lds(kernel, lds, cfg);
+  if (e != hipSuccess) return e;
+  int waves = p.k * at.waves;
+  const int route = KM ? (p.G + 63) / 64 : 1;               // a thread an agent
+  if (waves < route) waves = route > 16 ? 16 : route;
+  hipLaunchKernelGGL(kernel, dim3(p.n), dim3(waves * 64), lds, st, nd, m, p, at);
+  return hipGetLastError();
+}
+// the LDS of snap_row_kernel
+template <int BITS>
+static int row_lds(const SnapDesc &nd, int k, SnapLds &m, SnapRow &at) {
+  at.waves = waves_for(nd, 2, 16 / k);
+  at.lists = ddrl_roundup(nd.lay[0].in, 16) * 4;
+  at.y = at.lists + 16 * SNAP_MAXK * 12;
+  at.teams = at.y + ddrl_roundup(k * nd.A, 4) * 4;
+  at.team = lds_for<BITS, 1, 1, true>(nd, m);
+  return at.teams + k * at.team;
+}
 template <int BITS, int MT, bool STAGED>
 static hipError_t place_run(const SnapDesc &nd, const SnapMixture &p, hipStream_t st) {
   SnapLds m;
@@ -1198,7 +1413,7 @@ static hipError_t place_run(const SnapDesc &nd, const SnapMixture &p, hipStream_
   const auto kernel = snap_place_kernel<BITS, MT, STAGED>;
   hipError_t e = ddrl_set_lds(kernel, lds, cfg);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kernel, dim3(p.n * p.k), dim3(waves_for(nd, MT, 8) * 64), lds, st, nd, m, p);
+  hipLaunchKernelGGL(kernel, dim3(p.n * p.k), dim3(waves_for(nd, MT, STAGED ? 8 : 16) * 64), lds, st, nd, m, p);
   return hipGetLastError();
 }
 template <int BITS, int R, int NT, int MT, bool STAGED>
@@ -1235,17 +1450,29 @@ static hipError_t sort_run(const int *idx, int total, int G, int *sorted, int *s
   return hipGetLastError();
 }
 
+#define SNAP_ROUTE 32768             // agents x inputs up to which a row's workgroup is its own router
 #define SNAP_STATIC_LDS 2560         // snap_experts_kernel's lists
-extern "C" hipError_t snap_mixture_launch(const SnapDesc *nd, const SnapMixture *p, hipStream_t st) {
-  const int S = nd->lay[0].in, A = nd->A;
-  hipError_t e = p->k == 1 ? router_run<1>(*p, S, A, st) : p->k == 2 ? router_run<2>(*p, S, A, st) : p->k <= 4 ? router_run<4>(*p, S, A, st)
-                                                                                                              : router_run<8>(*p, S, A, st);
+static hipError_t router_launch(const SnapMixture &p, int S, int A, hipStream_t st) {
+  return p.k == 1 ? router_run<1>(p, S, A, st) : p.k == 2 ? router_run<2>(p, S, A, st) : p.k <= 4 ? router_run<4>(p, S, A, st) : router_run<8>(p, S, A, st);
+}
+template <int BITS>
+static hipError_t mixture_few(const SnapDesc &nd, const SnapMixture &p, hipStream_t st) {
+  const int S = nd.lay[0].in, A = nd.A;
+  SnapLds m;
+  SnapRow at;
+  const int lds = row_lds<BITS>(nd, p.k, m, at);
+  const bool together = lds <= SNAP_LDS - 1024;
+  if (together && (long long)p.G * S <= SNAP_ROUTE) return p.k <= 4 ? row_run<BITS, 4>(nd, p, m, at, lds, st) : row_run<BITS, 8>(nd, p, m, at, lds, st);
+  hipError_t e = router_launch(p, S, A, st);
   if (e != hipSuccess) return e;
+  if (together) return row_run<BITS, 0>(nd, p, m, at, lds, st);
+  return fits<BITS, 1, 1, true>(nd, SNAP_HALF) ? place_run<BITS, 2, true>(nd, p, st) : place_run<BITS, 2, false>(nd, p, st);
+}
+extern "C" hipError_t snap_mixture_launch(const SnapDesc *nd, const SnapMixture *p, hipStream_t st) {
   const int total = p->n * p->k, left = SNAP_LDS - SNAP_STATIC_LDS;
-  if (total <= SNAP_FEW) {
-    if (nd->bits == 4) return fits<4, 1, 1, true>(*nd, SNAP_HALF) ? place_run<4, 2, true>(*nd, *p, st) : place_run<4, 2, false>(*nd, *p, st);
-    return fits<32, 1, 1, true>(*nd, SNAP_HALF) ? place_run<32, 2, true>(*nd, *p, st) : place_run<32, 2, false>(*nd, *p, st);
-  }
+  if (total <= SNAP_FEW) return nd->bits == 4 ? mixture_few<4>(*nd, *p, st) : mixture_few<32>(*nd, *p, st);
+  hipError_t e = router_launch(*p, nd->lay[0].in, nd->A, st);
+  if (e != hipSuccess) return e;
   if ((e = sort_run(p->idx, total, p->G, p->sorted, p->start, st)) != hipSuccess) return e;
   if (nd->bits == 4) {
     if (fits<4, 16, 1, true>(*nd, left)) return experts_run<4, 16, 1, 2, true>(*nd, *p, st);
