@@ -177,27 +177,40 @@ __device__ __forceinline__ unsigned two_tops(float lo, float hi) { return __buil
 struct Team { int tid, threads, wave, waves; };
 __device__ __forceinline__ Team whole_team() { return {(int)threadIdx.x, (int)blockDim.x, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), (int)(blockDim.x >> 6)}; }
 
-// `rows(t)`: where row t of the tile lies, or null; all threads of the team, no barrier inside
-template <int BITS, int R, int NT, class Rows>
-__device__ __forceinline__ void tile_in(const Team &w, int K, char *buf, Rows rows) {
+// `rows(t)`: where row t of the tile lies, or null; `some`: any address that can be read, so that every load is unconditional and
+// BATCH are on their way at once.  All threads of the team, no barrier inside.
+template <int BITS, int R, int NT, int BATCH, class Rows>
+__device__ __forceinline__ void tile_in(const Team &w, int K, char *buf, const float *some, Rows rows) {
   using S = SnapShape<BITS, R, NT>;
   const int Kp = BITS == 4 ? (K + 31) & ~31 : (K + 15) & ~15;
   const int per = Kp <= 32 ? 32 : 64;                      // threads a row
-#pragma unroll 2
-  for (int t = w.tid / per; t < S::T; t += w.threads / per) {
-    const float *x = rows(t);
+  const int t0 = w.tid / per, dt = w.threads / per;
 #pragma unroll 1
-    for (int k = w.tid & (per - 1); k < Kp; k += per) {
-      float v = x && k < K ? x[k] : 0.f;
-      if (BITS == 4) {
-        v = v != v ? __uint_as_float(0x7fc00000u) : v;     // (a NaN that its upper half alone would not show)
-        float p[3];
-        split3(v, p);
+  for (int k = w.tid & (per - 1); k < Kp; k += per)
+#pragma unroll 1
+    for (int t1 = t0; t1 < S::T; t1 += BATCH * dt) {
+      float v[BATCH];
 #pragma unroll
-        for (int j = 0; j < 3; ++j) *(unsigned short *)(buf + S::at(t, j, k)) = bf_top(p[j]);
-      } else *(float *)(buf + S::at(t, 0, k)) = v;
+      for (int i = 0; i < BATCH; ++i) {
+        const int t = t1 + i * dt;
+        const float *x = t < S::T ? rows(t) : nullptr;
+        const bool ok = x && k < K;
+        v[i] = *(ok ? x + k : some);
+        v[i] = ok ? v[i] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int t = t1 + i * dt;
+        if (t >= S::T) break;
+        if (BITS == 4) {
+          const float z = v[i] != v[i] ? __uint_as_float(0x7fc00000u) : v[i];     // (a NaN that its upper half alone would not show)
+          float p[3];
+          split3(z, p);
+#pragma unroll
+          for (int j = 0; j < 3; ++j) *(unsigned short *)(buf + S::at(t, j, k)) = bf_top(p[j]);
+        } else *(float *)(buf + S::at(t, 0, k)) = v[i];
+      }
     }
-  }
 }
 
 // The barrier between layers: LDS is handed over, the weights already asked for stay in flight across it
@@ -540,7 +553,7 @@ snap_forward_kernel(const SnapDesc nd_, const SnapLds m, const SnapForward p) {
   for (int t0 = from; t0 < to; t0 += S::T) {
     net.ask(nd);
     const float *x = p.x + g * p.x_agent + t0 * p.x_row;
-    tile_in<BITS, R, NT>(net.w, nd->lay[0].in, lds, [&](int t) { return t0 + t < to ? x + t * p.x_row : (const float *)nullptr; });
+    tile_in<BITS, R, NT, (R > 1 && STAGED ? 2 : 1)>(net.w, nd->lay[0].in, lds, p.x, [&](int t) { return t0 + t < to ? x + t * p.x_row : (const float *)nullptr; });
     float *o = p.out + g * p.out_agent + t0 * p.out_row;
     net.tile(nd, m, lds, [&](int t, int n, float v) { if (t0 + t < to) o[t * p.out_row + n] = v; });
   }
@@ -921,7 +934,7 @@ snap_row_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p, const 
   SnapNet<BITS, 1, 1, MT, true> net(w);
   if (e >= 0) {
     net.stage(nd, m, p.img + (size_t)e * nd->stride, own);
-    tile_in<BITS, 1, 1>(w, S, own, [&](int) { return xs; });
+    tile_in<BITS, 1, 1, 1>(w, S, own, xs, [&](int) { return xs; });
   }
   if (tid < p.k && (KM || p.chunks > 1)) { p.idx[row * p.k + tid] = picks[tid]; p.prob[row * p.k + tid] = probs[tid]; }
   net.tile(nd, m, own, [&](int, int n, float v) { y[j * A + n] = v; });
@@ -965,7 +978,7 @@ snap_place_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
   net.stage(nd, m, p.img + (size_t)e * nd->stride, lds);
   net.ask(nd);
   const float *x = p.x + row * p.x_row;
-  tile_in<BITS, 1, 1>(net.w, nd->lay[0].in, lds, [&](int) { return x; });
+  tile_in<BITS, 1, 1, 1>(net.w, nd->lay[0].in, lds, p.x, [&](int) { return x; });
   net.tile(nd, m, lds, [&](int, int n, float v) { __hip_atomic_store(y + n, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
@@ -1033,7 +1046,7 @@ snap_sort_kernel(const int *__restrict__ idx, int total, int G, int bits, int *_
   extern __shared__ __align__(16) char lds[];
   sort_block(idx, blockIdx.x, total, G, bits, sorted, start, lds);
 }
-// A net's places (or, e = G, those that picked nobody) in up to 256 blocks from b0 on, as one list
+// An agent's places (or, e = G, those that picked nobody) in up to 256 blocks from b0 on, as one list
 struct Segments { int pre[257], at[256]; };
 __device__ __forceinline__ int segments_of(Segments &g, const int *start, int total, int G, int e, int b0, int blocks) {
   // all threads of a workgroup of 256 or more; barriers inside
@@ -1073,39 +1086,55 @@ __device__ __forceinline__ int place_of(const Segments &g, const int *sorted, in
 // The picked nets, many places: a workgroup answers, for one net, every gridDim.y-th tile of T of the places that picked it; the
 // rows are summed up as above.
 // ------------------------------------------------------------------------------------------------------------------------
-template <int BITS, int R, int NT, int MT, bool STAGED>
+template <int BITS, int R, int NT, int MT>
 __global__ void __launch_bounds__(512)
 snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
   extern __shared__ __align__(16) char lds[];
   using S = SnapShape<BITS, R, NT>;
-  __shared__ Segments seg;
-  __shared__ int list[S::T], done[S::T];
+  __shared__ int list[S::T], picked[S::T], done[S::T], have;
+  __shared__ float probs[S::T][SNAP_MAXK];
   const DescP nd = SNAP_DESC(nd_);
   const int tid = threadIdx.x, A = nd->A, threads = blockDim.x, e = blockIdx.x;
-  SnapNet<BITS, R, NT, MT, STAGED> net(whole_team());
-  bool staged = false;
-  for (int b0 = 0; b0 < p.blocks; b0 += 256) {
-    const int have = segments_of(seg, p.start, p.n * p.k, p.G, e, b0, min(256, p.blocks - b0));
-    for (int i0 = blockIdx.y * S::T; i0 < have; i0 += gridDim.y * S::T) {
-      if (!staged) { net.stage(nd, m, p.img + (size_t)e * nd->stride, lds); staged = true; }
-      net.ask(nd);
-      if (tid < S::T) list[tid] = i0 + tid < have ? place_of(seg, p.sorted, i0 + tid) : -1;
+  SnapNet<BITS, R, NT, MT, false> net(whole_team());
+  net.stage(nd, m, p.img + (size_t)e * nd->stride, lds);
+  for (int b0 = 0; b0 < p.blocks; b0 += 64) {
+    const int nb = min(64, p.blocks - b0);
+    int from = 0, cnt = 0;                                 // lane b of the first wave: the net's places in block b0 + b
+    if (tid < nb) {
+      const int *st = p.start + (int64_t)(b0 + tid) * (p.G + 1) + e;
+      from = st[0]; cnt = st[1] - from;
+      from += (b0 + tid) * SORT_BLOCK;
+    }
+    for (int i0 = blockIdx.y * S::T; ; i0 += gridDim.y * S::T) {
+      if (net.w.wave == 0) {
+        int at = -1, sum = 0;
+        for (int b = 0; b < nb; ++b) {
+          const int n = __builtin_amdgcn_readlane(cnt, b), f = __builtin_amdgcn_readlane(from, b), i = i0 + tid - sum;
+          at = i >= 0 && i < n ? f + i : at;
+          sum += n;
+        }
+        if (tid < S::T) list[tid] = at >= 0 ? p.sorted[at] : -1;
+        if (tid == 0) have = sum;
+      }
       __syncthreads();
-      tile_in<BITS, R, NT>(net.w, nd->lay[0].in, lds, [&](int t) { return list[t] >= 0 ? p.x + (int64_t)(list[t] / p.k) * p.x_row : (const float *)nullptr; });
+      if (i0 >= have) break;
+      net.ask(nd);
+      tile_in<BITS, R, NT, (R > 1 ? 4 : 1)>(net.w, nd->lay[0].in, lds, p.x, [&](int t) { return list[t] >= 0 ? p.x + (int64_t)(list[t] / p.k) * p.x_row : (const float *)nullptr; });
+      for (int i = tid; i < S::T * SNAP_MAXK; i += threads) {          // (wanted at the end)
+        const int t = i / SNAP_MAXK, j = i % SNAP_MAXK, r = list[t] / p.k;
+        const bool has = list[t] >= 0 && j < p.k;
+        probs[t][j] = has ? p.prob[r * p.k + j] : 0.f;
+        const unsigned long long who = __ballot(has && p.idx[has ? r * p.k + j : 0] >= 0);
+        if (j == 0) picked[t] = (int)(who >> (i & 63)) & 255;
+      }
       net.tile(nd, m, lds, [&](int t, int n, float v) {
         if (list[t] >= 0) __hip_atomic_store(p.y + (int64_t)list[t] * A + n, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       });
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       if (tid < S::T) {
-        int row = -1;
-        if (list[tid] >= 0) {
-          const int r = list[tid] / p.k;
-          int want = 0;
-          for (int j = 0; j < p.k; ++j) want += p.idx[r * p.k + j] >= 0;
-          if (__hip_atomic_fetch_add(p.count + r, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == want - 1) row = r;
-        }
-        done[tid] = row;
+        const int r = list[tid] / p.k;
+        done[tid] = list[tid] >= 0 && __hip_atomic_fetch_add(p.count + r, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == __popc(picked[tid]) - 1 ? r : -1;
       }
       __syncthreads();
       for (int i = tid; i < S::T * A; i += threads) {
@@ -1113,12 +1142,12 @@ snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
         if (r < 0) continue;
         float sum = 0.f;
         for (int j = 0; j < p.k; ++j)
-          if (p.idx[r * p.k + j] >= 0)
-            sum = fmaf(p.prob[r * p.k + j], __hip_atomic_load(p.y + ((int64_t)r * p.k + j) * A + a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), sum);
+          if (picked[t] >> j & 1) sum = fmaf(probs[t][j], __hip_atomic_load(p.y + ((int64_t)r * p.k + j) * A + a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), sum);
         p.out[r * p.out_row + a] = sum;
       }
       __syncthreads();
     }
+    __syncthreads();
   }
 }
 
@@ -1375,7 +1404,10 @@ static hipError_t router_run(const SnapMixture &p, int S, int A, hipStream_t st)
   const int ld = ddrl_roundup(S, 64) + 4;
   const int strips = ((p.G + 15) / 16 + p.chunks - 1) / p.chunks;
   int waves = 4;
-  while (waves < 16 && waves < strips) waves *= 2;
+  // with enough workgroups, fewer waves with more agents each have fewer lists to merge (256 agents of 45 inputs, 16384 rows: 8
+  // waves 24.6 us, 16 33.2; 4096 rows 9.6 and 9.4; 1024 agents, 512 rows 23.5 and 19.4)
+  const int most = p.n >= 8192 ? 8 : 16;
+  while (waves < most && waves < strips) waves *= 2;
   const size_t lds = (size_t)16 * ld * 4 + (size_t)16 * waves * KM * 12;
   static LdsConfig cfg;
   hipError_t e = ddrl_set_lds(snap_router_kernel<KM>, lds, cfg);
@@ -1416,21 +1448,21 @@ static hipError_t place_run(const SnapDesc &nd, const SnapMixture &p, hipStream_
   hipLaunchKernelGGL(kernel, dim3(p.n * p.k), dim3(waves_for(nd, MT, STAGED ? 8 : 16) * 64), lds, st, nd, m, p);
   return hipGetLastError();
 }
-template <int BITS, int R, int NT, int MT, bool STAGED>
+template <int BITS, int R, int NT, int MT>
 static hipError_t experts_run(const SnapDesc &nd, const SnapMixture &p, hipStream_t st) {
   SnapLds m;
-  const int lds = lds_for<BITS, R, NT, STAGED>(nd, m);
+  const int lds = lds_for<BITS, R, NT, false>(nd, m);
   static LdsConfig cfg;
-  const auto kernel = snap_experts_kernel<BITS, R, NT, MT, STAGED>;
+  const auto kernel = snap_experts_kernel<BITS, R, NT, MT>;
   hipError_t e = ddrl_set_lds(kernel, lds, cfg);
   if (e != hipSuccess) return e;
   int waves = waves_for(nd, MT, 8);
   waves = waves < 4 ? 4 : waves;
   // Several workgroups a net, each every share-th of its tiles: a router prefers some nets, and a net's tiles one after the other
-  // are what a pass then waits for (256 nets, 4096 rows, top 2: 53 us with 2 workgroups a net, 25 us with 8); a workgroup that
-  // finds no tile is over after two reads.
+  // are what a pass then waits for (1024 agents of 45-64-64-17, 8192 rows, top 4: 77 us with 2 workgroups a net, 60 with 4; 256
+  // agents, 4096 rows, top 2: 53 with 2 and 21 with 8 or 16); a workgroup that finds no tile is over after two reads.
   const int64_t total = (int64_t)p.n * p.k, T = R * NT;
-  int64_t share = (2048 + p.G - 1) / p.G;
+  int64_t share = (4096 + p.G - 1) / p.G;
   const int64_t tiles = (total + T - 1) / T;
   if (share > tiles) share = tiles;
   hipLaunchKernelGGL(kernel, dim3(p.G, (unsigned)share), dim3(waves * 64), lds, st, nd, m, p);
@@ -1450,8 +1482,10 @@ static hipError_t sort_run(const int *idx, int total, int G, int *sorted, int *s
   return hipGetLastError();
 }
 
-#define SNAP_ROUTE 32768             // agents x inputs up to which a row's workgroup is its own router
-#define SNAP_STATIC_LDS 2560         // snap_experts_kernel's lists
+// agents x inputs up to which a row's workgroup is its own router (64-64 nets, top 2, 8 or 64 rows: 1024 agents of 45 inputs 11.6 us,
+// with a router of its own 15.3; 256 of 376 15.6 and 28.7; 1024 of 128 22.0 and 17.9)
+#define SNAP_ROUTE 98304
+#define SNAP_STATIC_LDS 2048         // snap_experts_kernel's lists
 static hipError_t router_launch(const SnapMixture &p, int S, int A, hipStream_t st) {
   return p.k == 1 ? router_run<1>(p, S, A, st) : p.k == 2 ? router_run<2>(p, S, A, st) : p.k <= 4 ? router_run<4>(p, S, A, st) : router_run<8>(p, S, A, st);
 }
@@ -1474,14 +1508,18 @@ extern "C" hipError_t snap_mixture_launch(const SnapDesc *nd, const SnapMixture 
   hipError_t e = router_launch(*p, nd->lay[0].in, nd->A, st);
   if (e != hipSuccess) return e;
   if ((e = sort_run(p->idx, total, p->G, p->sorted, p->start, st)) != hipSuccess) return e;
+  // From memory to registers, not staged (16 agents of 18-100-100-6, 1024 rows, 32 bits: 20.7 us, staged 25.3; 256 of 45-64-64-17,
+  // 4096 rows: the same).  Very many places of nets that leave two workgroups a CU go in tiles of 32 rows (256 agents of 45-64-64-17,
+  // 16384 rows: 93 us, in tiles of 16 109; 4096 rows 34.0 and 35.9; 2048 rows 28.1 and 26.1; 64 of 18-400-300-6, 4096 rows 109 and 103).
+  const bool many = total >= 8192;
   if (nd->bits == 4) {
-    if (fits<4, 16, 1, true>(*nd, left)) return experts_run<4, 16, 1, 2, true>(*nd, *p, st);
-    if (fits<4, 16, 1, false>(*nd, left)) return experts_run<4, 16, 1, 1, false>(*nd, *p, st);
-    return experts_run<4, 4, 1, 1, false>(*nd, *p, st);
+    if (many && fits<4, 16, 2, false>(*nd, SNAP_HALF)) return experts_run<4, 16, 2, 1>(*nd, *p, st);
+    if (fits<4, 16, 1, false>(*nd, left)) return experts_run<4, 16, 1, 1>(*nd, *p, st);
+    return experts_run<4, 4, 1, 1>(*nd, *p, st);
   }
-  if (fits<32, 16, 1, true>(*nd, left)) return experts_run<32, 16, 1, 1, true>(*nd, *p, st);
-  if (fits<32, 16, 1, false>(*nd, left)) return experts_run<32, 16, 1, 1, false>(*nd, *p, st);
-  return experts_run<32, 1, 1, 2, false>(*nd, *p, st);
+  if (many && fits<32, 16, 2, false>(*nd, SNAP_HALF)) return experts_run<32, 16, 2, 1>(*nd, *p, st);
+  if (fits<32, 16, 1, false>(*nd, left)) return experts_run<32, 16, 1, 1>(*nd, *p, st);
+  return experts_run<32, 1, 1, 2>(*nd, *p, st);
 }
 
 template <int KM>
