@@ -1518,8 +1518,7 @@ extern "C" hipError_t snap_mixture_launch(const SnapDesc *nd, const SnapMixture 
     return experts_run<4, 4, 1, 1>(*nd, *p, st);
   }
   if (many && fits<32, 16, 2, false>(*nd, SNAP_HALF)) return experts_run<32, 16, 2, 1>(*nd, *p, st);
-  if (fits<32, 16, 1, false>(*nd, left)) return experts_run<32, 16, 1, 1>(*nd, *p, st);
-  return experts_run<32, 1, 1, 2>(*nd, *p, st);
+  return experts_run<32, 16, 1, 1>(*nd, *p, st);                        // (fits whatever the net: 128 KiB at most)
 }
 
 template <int KM>

@@ -242,7 +242,7 @@ extern "C" int ddrl_snap_get_weights(ddrl_snap_t *s, double *flat) {
 }
 
 static int forward_on(ddrl_snap *s, const ddrl_snap_forward_args *a, hipStream_t st) {
-  if (a->n < 0) return ddrl_fail(DDRL_EINVAL, "n=%d < 0", a->n);
+  if (a->n < 0 || a->n > (1 << 28)) return ddrl_fail(DDRL_EINVAL, "n=%d: 0..%d", a->n, 1 << 28);
   if (a->n == 0) return DDRL_OK;
   if (!a->x || !a->out || off4(a->x) || off4(a->out)) return ddrl_fail(DDRL_EINVAL, "x / out NULL or misaligned");
   const int64_t S = s->nd.lay[0].in, A = s->nd.A, n = a->n, G = s->G;

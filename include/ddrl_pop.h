@@ -597,7 +597,7 @@ int ddrl_snap_get_weights(ddrl_snap_t *s, double *flat);
 
 /* every agent's net on n rows: x [n_agents x n x in_dim] -> out [n_agents x n x out_dim] */
 typedef struct {
-  int n;                                   /* rows per agent, >= 0 */
+  int n;                                   /* rows per agent, 0..2^28 */
   const float *x;
   int64_t x_agent, x_row;                  /* x_agent 0: all agents read the same n rows; x_row 0: an agent's rows are one row */
   float *out;
@@ -617,7 +617,7 @@ int ddrl_snap_forward(ddrl_snap_t *s, int n, const float *x, float *out);
  * Where fewer than top_k are left, the last places of idx hold -1, of prob and y 0; a row with none has out = 0.
  * n * top_k of 256 and more, here and in the gradient: up to 16383 agents. */
 typedef struct {
-  int n, top_k;                            /* rows >= 0; 1 <= top_k <= min(DDRL_SNAP_MAX_TOP_K, n_agents) */
+  int n, top_k;                            /* rows >= 0; 1 <= top_k <= min(DDRL_SNAP_MAX_TOP_K, n_agents); n * top_k <= 2^28 */
   const float *x; int64_t x_row;           /* [n x in_dim] */
   const float *router_w; int64_t router_row;   /* [n_agents x in_dim] */
   const float *router_b;                   /* [n_agents] or NULL */
