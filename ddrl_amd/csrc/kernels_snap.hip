@@ -68,44 +68,60 @@ snap_load_kernel(const SnapDesc nd_, const SnapSource src, char *__restrict__ im
   const float *b = src.w + (size_t)blockIdx.x * src.agent + from->offb[l];
   char *rec = img + (size_t)blockIdx.x * nd->stride + y.off + strip * y.rec;
   const int kp = from->kp[l];
-  auto weight = [&](int k) -> float {
-    if (n >= N || k >= K) return 0.f;
-    return src.tiled ? w[ddrl_widx(n, k, kp)] : w[(size_t)n * K + k];
+  // inputs k .. k + 3, k a multiple of 4 (four neighbours in memory in a tile too), zeros where there are none
+  auto four = [&](int k) -> f32x4 {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (n >= N || k >= K) return v;
+    const float *from = w + (src.tiled ? (size_t)ddrl_widx(n, k, kp) : (size_t)n * K + k);
+    if (k + 4 <= K) return *(const f32x4u *)from;
+    for (int i = 0; i < 3; ++i) if (k + i < K) v[i] = from[i];
+    return v;
   };
   bool bad = false;
   if (nd->bits == 4) {
-    for (int s = 0; s < steps; ++s) {
-      float v[8], amax = 0.f;
-      bool wild = false;
+#pragma unroll 1
+    for (int s0 = 0; s0 < steps; s0 += 4) {
+      f32x4 v[4][2];
+      u32x4 codes;
+      unsigned scales = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = weight(32 * s + 8 * q + i);
-        const float a = fabsf(v[i]);
-        wild = wild || !(a < 0x1p126f);
-        amax = fmaxf(amax, a);
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) v[s][h] = four(32 * (s0 + s) + 8 * q + 4 * h);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        float amax = 0.f;
+        bool wild = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float a = fabsf(v[s][i >> 2][i & 3]);
+          wild = wild || !(a < 0x1p126f);
+          amax = fmaxf(amax, a);
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 16)); amax = fmaxf(amax, __shfl_xor(amax, 32));
+        int any = wild ? 1 : 0;
+        any |= __shfl_xor(any, 16); any |= __shfl_xor(any, 32);
+        bad = bad || any;
+        const unsigned bits = __float_as_uint(amax);
+        const int e = (int)(bits >> 23) - 127, sh = (bits & 0x7fffffu) <= 0x400000u ? e - 2 : e - 1;
+        const bool none = any || amax < 0x1p-118f;
+        const float inv = none ? 0.f : __uint_as_float((unsigned)(127 - sh) << 23);
+        unsigned c = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c |= (none ? 0u : snap_code(v[s][i >> 2][i & 3] * inv)) << (4 * i);
+        codes[s] = c;
+        scales |= (unsigned)(none ? 127 : sh + 127) << (8 * s);
       }
-      amax = fmaxf(amax, __shfl_xor(amax, 16)); amax = fmaxf(amax, __shfl_xor(amax, 32));
-      int any = wild ? 1 : 0;
-      any |= __shfl_xor(any, 16); any |= __shfl_xor(any, 32);
-      bad = bad || any;
-      const unsigned bits = __float_as_uint(amax);
-      const int e = (int)(bits >> 23) - 127, sh = (bits & 0x7fffffu) <= 0x400000u ? e - 2 : e - 1;
-      const bool none = any || amax < 0x1p-118f;
-      const float inv = none ? 0.f : __uint_as_float((unsigned)(127 - sh) << 23);
-      unsigned c = 0;
+      if (s0 + 4 <= steps) *(u32x4 *)(rec + snap_code_off(steps, s0, lane)) = codes;
+      else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c |= (none ? 0u : snap_code(v[i] * inv)) << (4 * i);
-      *(unsigned *)(rec + snap_code_off(steps, s, lane)) = c;
-      if (q == 0) rec[snap_scale_off(y.code, s, r)] = (char)(none ? 127 : sh + 127);
+        for (int s = 0; s < 3; ++s) if (s0 + s < steps) *(unsigned *)(rec + snap_code_off(steps, s0 + s, lane)) = codes[s];
+      }
+      if (q == 0) *(unsigned *)(rec + snap_scale_off(y.code, s0, r)) = scales;
     }
-    if (q == 0) for (int s = steps; s & 3; ++s) rec[snap_scale_off(y.code, s, r)] = 127;
   } else {
-    for (int s = 0; s < steps; ++s) {
-      f32x4 v;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = weight(16 * s + 4 * q + i);
-      *(f32x4 *)(rec + s * 1024 + lane * 16) = v;
-    }
+#pragma unroll 4
+    for (int s = 0; s < steps; ++s) *(f32x4 *)(rec + s * 1024 + lane * 16) = four(16 * s + 4 * q);
   }
   if (q == 0) ((float *)(rec + y.rec - 64))[r] = n >= N ? 0.f : bad ? __uint_as_float(0x7fc00000u) : b[n];
 }
