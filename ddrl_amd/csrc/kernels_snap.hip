@@ -46,7 +46,8 @@ __device__ __forceinline__ f32x4 act_four(int act, f32x4 x) {
 // Loading.  One wave per (agent, layer, strip): lane (r, q) walks the k-steps of output r; the four lanes of an output agree
 // on a block's largest magnitude.  With amax = m 2^e, m in [1, 2): amax <= 6 2^s for the least s = e - 2 (m <= 1.5) or e - 1,
 // so the scale comes out of the exponent field alone, and w 2^-s is exact: the codes do not depend on any rounding of the
-// machine's.  Bound by the reads of the fp32 parameters.
+// machine's.  Bound by the reads of the fp32 parameters, 16 bytes a lane and a block of four steps at a time (1024 agents of
+// 18-400-300-6 to 4 bits, 530 MB: 197 us, 2.7 TB/s; a wave's blocks come one after the other).
 // ------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ unsigned snap_code(float v) {          // v = w / scale, |v| <= 6: nearest of the grid, halves to the even code
   const float a = fabsf(v);
@@ -148,7 +149,10 @@ extern "C" hipError_t snap_load_launch(const SnapDesc *nd, char *img, const Snap
 // finishing four: with few rows that, not the product, is most of the instructions.
 // Activations lie as the B operand is read, [k-step][part][16 rows][k quarter][row] x 16 bytes: a wave's read is 1 KiB without a
 // bank conflict, every one of a block of steps at a constant distance from the first.  Instructions, not bytes, bound a net
-// of many rows, so what is left of addresses is a scalar or such a constant.
+// of many rows, so what is left of addresses is a scalar or such a constant (1024 agents of 18-400-300-6, 64 rows: 96 us, 530
+// TFLOP/s of the three bf16 products; 147 us with 7 vector instructions a product and row-major inputs.  A wave of several strips or
+// tiles at once shares more, and leaves waves idle where a layer ends: 110 to 196 us).  One row is bound by its net's bytes
+// and by the layers' latency, some 3000 cycles each (84 MB of them: 21.4 us, 3.9 TB/s).
 // ------------------------------------------------------------------------------------------------------------------------
 struct SnapLds { int second, image; };          // the inputs of layers 0, 2 lie in the first LDS buffer, those of 1, 3 in the second; behind them the image, where it is staged
 
@@ -580,7 +584,8 @@ snap_forward_kernel(const SnapDesc nd_, const SnapLds m, const SnapForward p) {
 // v_mfma_f64_16x16x4_f64.  Both factors are 32-bit numbers, so their products are exact and the sums are wrong by ~1e-16: two
 // logits change places only where they are equal to 15 digits.  A lane holds 4 logits of one row a strip and keeps the KM best
 // it has met, as keys that sort as the numbers do (NaN above all, 0 = barred); the lanes of a row, then the waves, merge their
-// lists.  The index decides between equal keys.
+// lists.  The index decides between equal keys.  Bound by latency: one strip a wave, then the lists (256 agents, 4096 rows of 45: 9.4
+// us, 10 TFLOP/s).
 // ------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ unsigned long long logit_key(double v) {
   if (v != v) return ~0ull;
@@ -844,7 +849,8 @@ __device__ __forceinline__ void row_picks(const SnapMixture &p, int row, int *pi
 // Few rows, nets that fit in LDS together: a workgroup a row, a team of its waves for each pick, so that the answers meet in LDS.
 // And as long as the router's matrix is small, every workgroup works the router out for its row by itself (KM > 0), a thread an
 // agent at a time, sums in fp64 as above: one launch, nothing to hand over.  Bound by the latency of what follows on what: the
-// router's rows, the picks, the nets' images, the layers.
+// router's rows, the picks, the nets' images, the layers (16 agents of 18-100-100-6 in 32 bits, one row, top 2: 8.5 us; router and
+// nets in two launches: 11.9.  1024 in 4 bits, 8 rows, top 4: 14.2 and 18.7).
 // ------------------------------------------------------------------------------------------------------------------------
 // inputs at .. at + 3 of a router row of S, zeros behind its end; no lane reads beyond it
 __device__ __forceinline__ f32x4 row_four(const float *w, int at, int S) {
@@ -969,7 +975,8 @@ snap_row_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p, const 
 // Few places of larger nets: a workgroup for each.  Whoever answers a row's last place sums the row up, in the order of its places
 // whatever the order they were answered in.  The answers are stored past the XCD's own cache (agent scope); once they have arrived
 // the counter may tell of them.  Nothing else passes between workgroups, so no cache has to be written back or forgotten, and
-// nobody waits.
+// nobody waits.  Bound by what one CU has in flight from memory (66 places of 18-400-300-6 in 32 bits, 34 MB: 15 us, 13 waves each;
+// with 8 waves 17 us).
 // ------------------------------------------------------------------------------------------------------------------------
 template <int BITS, int MT, bool STAGED>
 __global__ void __launch_bounds__(STAGED ? 512 : 1024)
@@ -1016,7 +1023,7 @@ snap_place_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
 // ------------------------------------------------------------------------------------------------------------------------
 // Who picked a net, when there are many places: every 1024 places of idx sorted by the net they picked, in their order.  Lanes of a
 // wave with the same net find each other bit by bit; the waves take their turns at the nets' counters, so that a place's position
-// does not hang on who came first.  Places that picked nobody go to net G.
+// does not hang on who came first.  Places that picked nobody go to net G.  Bound by that chain: 4.7 us for 8192 places, 5.0 for 32768.
 // ------------------------------------------------------------------------------------------------------------------------
 #define SORT_BLOCK 1024
 __device__ __forceinline__ void sort_block(const int *__restrict__ idx, int block, int total, int G, int bits, int *__restrict__ sorted, int *__restrict__ start, char *lds) {
@@ -1100,7 +1107,8 @@ __device__ __forceinline__ int place_of(const Segments &g, const int *sorted, in
 
 // ------------------------------------------------------------------------------------------------------------------------
 // The picked nets, many places: a workgroup answers, for one net, every gridDim.y-th tile of T of the places that picked it; the
-// rows are summed up as above.
+// rows are summed up as above.  Bound by what follows on what in a tile (its places, their inputs, the layers, the answers' way to
+// memory and back), some 8 us: 256 agents of 45-64-64-17, 4096 rows, top 2, 32 bits 20.5 us.
 // ------------------------------------------------------------------------------------------------------------------------
 template <int BITS, int R, int NT, int MT>
 __global__ void __launch_bounds__(512)
@@ -1174,7 +1182,8 @@ snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
 // Many: a first launch takes all dlogits and, in other workgroups, sorts the places by agent; in a second one a workgroup per agent
 // sums over the places that picked it, in their order, a wave every fourth of them and a lane an input.  Few agents: several
 // workgroups each, a run of sorted blocks every one; their sums go to the workspace, and the last of them adds all, in order.
-// Sums over rows are in fp64 (an agent may be picked by every row).
+// Sums over rows are in fp64 (an agent may be picked by every row).  Bound by launches and latency: 16 agents of 18 inputs, 9 rows,
+// top 2: 4.1 us; 1024 of 45, 4096 rows, top 4: 5.9 and 6.3 us (sums by the workgroup of an agent over unsorted idx: 65).
 // ------------------------------------------------------------------------------------------------------------------------
 // dlogit of a place, in all of its 16 lanes (a0 = 0 .. 15), and dy; one that picked nobody: 0
 template <int KM>
