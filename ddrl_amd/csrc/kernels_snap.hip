@@ -583,7 +583,7 @@ snap_forward_kernel(const SnapDesc nd_, const SnapLds m, const SnapForward p) {
 // The router.  One workgroup per 16 rows; a wave takes strips of 16 agents: logits[16 agents x 16 rows] on
 // v_mfma_f64_16x16x4_f64.  Both factors are 32-bit numbers, so their products are exact and the sums are wrong by ~1e-16: two
 // logits change places only where they are equal to 15 digits.  A lane holds 4 logits of one row a strip and keeps the KM best
-// it has met, as keys that sort as the numbers do (NaN above all, 0 = barred); the lanes of a row, then the waves, merge their
+// it has met, as keys that sort as the numbers do (NaN above all, a barred one as -infinity); the lanes of a row, then the waves, merge their
 // lists.  The index decides between equal keys.  Bound by latency: one strip a wave, then the lists (256 agents, 4096 rows of 45: 9.4
 // us, 10 TFLOP/s).
 // ------------------------------------------------------------------------------------------------------------------------
@@ -727,7 +727,7 @@ __device__ __forceinline__ float pick_prob(unsigned long long mk, int mi) {
   return mi != IDX_NONE ? ex / sum : 0.f;
 }
 
-// grid (rows / 16, chunks): the rows' best among the agents [chunk * G / chunks, ..); with one chunk the picks themselves
+// grid (rows / 16, chunks): the rows' best among the chunk's agents; with one chunk the picks themselves
 template <int KM>
 __global__ void __launch_bounds__(1024)
 snap_router_kernel(const SnapMixture p, int S, int A, int ld) {
@@ -1023,7 +1023,8 @@ snap_place_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
 // ------------------------------------------------------------------------------------------------------------------------
 // Who picked a net, when there are many places: every 1024 places of idx sorted by the net they picked, in their order.  Lanes of a
 // wave with the same net find each other bit by bit; the waves take their turns at the nets' counters, so that a place's position
-// does not hang on who came first.  Places that picked nobody go to net G.  Bound by that chain: 4.7 us for 8192 places, 5.0 for 32768.
+// does not hang on who came first.  Places that picked nobody go to net G.  Bound by the latency of a launch, a read and a write (4.7
+// us for 8192 places, 5.0 for 32768; a counter a wave instead of turns: the same).
 // ------------------------------------------------------------------------------------------------------------------------
 #define SORT_BLOCK 1024
 __device__ __forceinline__ void sort_block(const int *__restrict__ idx, int block, int total, int G, int bits, int *__restrict__ sorted, int *__restrict__ start, char *lds) {
@@ -1069,40 +1070,27 @@ snap_sort_kernel(const int *__restrict__ idx, int total, int G, int bits, int *_
   extern __shared__ __align__(16) char lds[];
   sort_block(idx, blockIdx.x, total, G, bits, sorted, start, lds);
 }
-// An agent's places (or, e = G, those that picked nobody) in up to 256 blocks from b0 on, as one list
-struct Segments { int pre[257], at[256]; };
-__device__ __forceinline__ int segments_of(Segments &g, const int *start, int total, int G, int e, int b0, int blocks) {
-  // all threads of a workgroup of 256 or more; barriers inside
-  __shared__ int wsum[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  __syncthreads();
-  int c = 0, sum = 0;
-  if (tid < 256) {
-    if (tid < blocks) {
-      const int *st = start + (int64_t)(b0 + tid) * (G + 1) + e;
-      const int from = st[0];
-      c = (e < G ? st[1] : min(SORT_BLOCK, total - (b0 + tid) * SORT_BLOCK)) - from;
-      g.at[tid] = (b0 + tid) * SORT_BLOCK + from;
-    }
-    sum = c;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) { const int o = __shfl_up(sum, d); sum += lane >= d ? o : 0; }
-    if (lane == 63) wsum[wave] = sum;
+// The i-th place of net e in the blocks b0 .. b0 + nb - 1 (nb <= 64), each thread of a wave its own i; `have`: how many there are.
+// Lane b holds block b0 + b's.
+struct Places { int from, cnt; };
+__device__ __forceinline__ Places places_of(const int *start, int G, int e, int b0, int nb, int lane) {
+  Places g = {0, 0};
+  if (lane < nb) {
+    const int *st = start + (int64_t)(b0 + lane) * (G + 1) + e;
+    g.cnt = st[1] - st[0];
+    g.from = (b0 + lane) * SORT_BLOCK + st[0];
   }
-  __syncthreads();
-  if (tid < 256) {
-    for (int w = 0; w < wave; ++w) sum += wsum[w];
-    g.pre[tid + 1] = sum;
-    if (tid == 0) g.pre[0] = 0;
-  }
-  __syncthreads();
-  return g.pre[256];
+  return g;
 }
-__device__ __forceinline__ int place_of(const Segments &g, const int *sorted, int i) {
-  int lo = 0;
-#pragma unroll
-  for (int d = 128; d; d >>= 1) lo += g.pre[lo + d] <= i ? d : 0;
-  return sorted[g.at[lo] + i - g.pre[lo]];
+__device__ __forceinline__ int place_at(const Places &g, int nb, int i, int &have) {
+  int at = -1;
+  have = 0;
+  for (int b = 0; b < nb; ++b) {
+    const int n = __builtin_amdgcn_readlane(g.cnt, b), f = __builtin_amdgcn_readlane(g.from, b);
+    at = i >= have && i < have + n ? f + i - have : at;
+    have += n;
+  }
+  return at;
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
@@ -1123,20 +1111,11 @@ snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
   net.stage(nd, m, p.img + (size_t)e * nd->stride, lds);
   for (int b0 = 0; b0 < p.blocks; b0 += 64) {
     const int nb = min(64, p.blocks - b0);
-    int from = 0, cnt = 0;                                 // lane b of the first wave: the net's places in block b0 + b
-    if (tid < nb) {
-      const int *st = p.start + (int64_t)(b0 + tid) * (p.G + 1) + e;
-      from = st[0]; cnt = st[1] - from;
-      from += (b0 + tid) * SORT_BLOCK;
-    }
+    const Places places = places_of(p.start, p.G, e, b0, nb, tid & 63);
     for (int i0 = blockIdx.y * S::T; ; i0 += gridDim.y * S::T) {
       if (net.w.wave == 0) {
-        int at = -1, sum = 0;
-        for (int b = 0; b < nb; ++b) {
-          const int n = __builtin_amdgcn_readlane(cnt, b), f = __builtin_amdgcn_readlane(from, b), i = i0 + tid - sum;
-          at = i >= 0 && i < n ? f + i : at;
-          sum += n;
-        }
+        int sum;
+        const int at = place_at(places, nb, i0 + tid, sum);
         if (tid < S::T) list[tid] = at >= 0 ? p.sorted[at] : -1;
         if (tid == 0) have = sum;
       }
@@ -1301,7 +1280,6 @@ snap_grad_first_kernel(const SnapGrad p, int bits) {
 template <int SJ>                                          // 64 SJ inputs
 __global__ void __launch_bounds__(256)
 snap_grad_sum_kernel(const SnapGrad p) {
-  __shared__ Segments seg;
   __shared__ int rows[256], last;
   __shared__ float dl[256];
   __shared__ double part[4][64];
@@ -1310,15 +1288,18 @@ snap_grad_sum_kernel(const SnapGrad p) {
 #pragma unroll
   for (int j = 0; j < SJ; ++j) acc[j] = 0.;
   const int b_from = blockIdx.y * p.piece, b_to = min(p.blocks, b_from + p.piece);
-  for (int b0 = b_from; b0 < b_to; b0 += 256) {
-    const int have = segments_of(seg, p.start, p.n * p.k, p.G, e, b0, min(256, b_to - b0));
+  for (int b0 = b_from; b0 < b_to; b0 += 64) {
+    const int nb = min(64, b_to - b0);
+    const Places places = places_of(p.start, p.G, e, b0, nb, lane);
+    int have = 1;
     for (int i0 = 0; i0 < have; i0 += 256) {
-      const int now = min(256, have - i0);
-      if (tid < now) {
-        const int place = place_of(seg, p.sorted, i0 + tid);
+      const int at = place_at(places, nb, i0 + tid, have);   // (the same `have` in every wave)
+      if (at >= 0) {
+        const int place = p.sorted[at];
         rows[tid] = place / p.k;
         dl[tid] = p.dlogit[place];
       }
+      const int now = min(256, have - i0);
       __syncthreads();
 #pragma unroll 8
       for (int i = wave; i < now; i += 4) {

@@ -8,7 +8,7 @@
 #define SNAP_MAXW 1024         // widest layer, as DDRL_WIDE_MAXW
 #define SNAP_MAXK 8            // DDRL_SNAP_MAX_TOP_K
 #define SNAP_LDS (160 * 1024)  // a CU's LDS
-#define SNAP_FEW 256           // places (rows x top_k) up to which a mixture answers each in a workgroup of its own
+#define SNAP_FEW 256           // places (rows x top_k) up to which a mixture gives every row, or every place, a workgroup of its own
 #define SNAP_CHUNK 256         // agents a router workgroup looks at when there are few rows
 
 // An agent's net is one image of `stride` bytes: its layers one after the other, a layer a row of records, one for 16 outputs
