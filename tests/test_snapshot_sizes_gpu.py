@@ -283,3 +283,48 @@ def test_calls_at_once(n):
     torch.cuda.synchronize()
     for (st, run, results), w in zip(made, want):
         assert all(np.array_equal(a, b) for a, b in zip(results(), w))
+
+
+# ---- what is left --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bits", [32, 4])
+def test_an_empty_snapshot_answers_what_zero_weights_answer(bits):
+    import ddrl_amd
+    for dims, n in (((18, 20, 6), 1), ((18, 20, 6), 3), ((18, 400, 300, 6), 17)):
+        s = ddrl_amd.PolicySnapshot.shaped(4, dims[0], dims[-1], dims[1:-1], bits=bits)
+        x = np.random.RandomState(1).uniform(-1, 1, (4, n, dims[0]))
+        assert (ask(s, x) == 0).all() and (s.weights() == 0).all()
+        out, idx, prob, _ = ask_mixture(s, x[0], np.zeros((4, dims[0]), np.float32), None, 3)
+        assert (out == 0).all() and (idx == [0, 1, 2]).all() and np.abs(prob - 1 / 3).max() <= sc.U
+
+
+@pytest.mark.parametrize("n", [3, 400])
+def test_logits_that_are_infinite(n):
+    """an infinite logit comes first; the softmax over it is what the formula gives, not a number"""
+    g, k = 30, 3
+    rng = np.random.RandomState(4)
+    s, layers = one_net(rng, g, (5, 9, 2), 32)
+    x = rng.uniform(0.5, 1, (n, 5)).astype(np.float32)
+    rw, rb = rng.standard_normal((g, 5)).astype(np.float32), rng.standard_normal(g).astype(np.float32)
+    rb[[7, 22]] = np.inf
+    out, idx, prob, y = ask_mixture(s, x, rw, rb, k)
+    assert (idx[:, :2] == [7, 22]).all() and np.isnan(prob).all() and np.isnan(out).all() and np.isfinite(y).all()
+    allowed = np.ones(g); allowed[[7, 22]] = 0
+    check_mixture(s, layers, x[:40], rw, rb, k, allowed)
+    rb[[7, 22]] = np.nan                                              # barred: whatever its logit is
+    check_mixture(s, layers, x[:40], rw, np.where(np.isnan(rb), -np.inf, rb).astype(np.float32), k)
+    a = ask_mixture(s, x, rw, rb, k, allowed)
+    b = ask_mixture(s, x, rw, np.where(np.isnan(rb), 0, rb).astype(np.float32), k, allowed)
+    assert all(np.array_equal(u, v) for u, v in zip(a, b))
+
+
+def test_rows_that_overlap_in_memory():
+    """inputs may: a sliding window over one series"""
+    s, layers = one_net(np.random.RandomState(5), 3, (18, 20, 6), 4)
+    series = np.random.RandomState(6).uniform(-1, 1, 50).astype(np.float32)
+    xd, out = dev(series), torch.zeros(3, 33, 6, device=DEV)
+    s.forward_dev(s.forward_args(33, xd.data_ptr(), out.data_ptr(), x_agent=0, x_row=1))
+    torch.cuda.synchronize()
+    x = np.lib.stride_tricks.sliding_window_view(series, 18)
+    want, bound = sc.forward(layers, np.broadcast_to(x, (3,) + x.shape), HIDDEN, LAST)
+    within(out.cpu().numpy(), want, bound)
