@@ -149,7 +149,7 @@ extern "C" hipError_t snap_load_launch(const SnapDesc *nd, char *img, const Snap
 // finishing four: with few rows that, not the product, is most of the instructions.
 // Activations lie as the B operand is read, [k-step][part][16 rows][k quarter][row] x 16 bytes: a wave's read is 1 KiB without a
 // bank conflict, every one of a block of steps at a constant distance from the first.  Instructions, not bytes, bound a net
-// of many rows, so what is left of addresses is a scalar or such a constant (1024 agents of 18-400-300-6, 64 rows: 96 us, 530
+// of many rows, so what is left of addresses is a scalar or such a constant (1024 agents of 18-400-300-6, 64 rows: 95 us, 530
 // TFLOP/s of the three bf16 products; 147 us with 7 vector instructions a product and row-major inputs.  A wave of several strips or
 // tiles at once shares more, and leaves waves idle where a layer ends: 110 to 196 us).  One row is bound by its net's bytes
 // and by the layers' latency, some 3000 cycles each (84 MB of them: 21.4 us, 3.9 TB/s).
@@ -559,7 +559,7 @@ template <int BITS, int R, int NT, int MT, bool STAGED> struct SnapNet {
 // Every agent's net on its rows
 // ------------------------------------------------------------------------------------------------------------------------
 template <int BITS, int R, int NT, int MT, bool STAGED>
-__global__ void __launch_bounds__(R == 16 && !STAGED ? 1024 : 512)
+__global__ void __launch_bounds__(R == 16 && !STAGED ? 1024 : 512, BITS == 4 && R == 16 && !STAGED ? 6 : 1)     // (6 waves a SIMD: see forward_run)
 snap_forward_kernel(const SnapDesc nd_, const SnapLds m, const SnapForward p) {
   extern __shared__ __align__(16) char lds[];
   using S = SnapShape<BITS, R, NT>;
@@ -1376,9 +1376,10 @@ static hipError_t forward_run(const SnapDesc &nd, SnapForward p, hipStream_t st)
   if (chunks > tiles) chunks = tiles;
   const int per = (tiles + chunks - 1) / chunks;
   p.per = per * R;
-  // 8 waves, so that two workgroups share a CU and one computes at the other's barriers; where the activations leave room for
-  // one only, 16 (1024 agents, 64 rows: 18-400-300-6 with 8 waves 105 us, with 16 132 us; 18-600-500-6 275 and 219 us)
-  const int most = R == 16 && !STAGED && lds > SNAP_HALF ? 16 : 8;
+  // 8 waves; tiles of 16 rows of larger nets 12 (4 bits: two workgroups of them fit a CU's registers), where the activations leave
+  // room for one workgroup a CU 16 (1024 agents, 64 rows: 18-400-300-6 with 8 waves 103 us, 12 97, 10 127, as 10 do not
+  // spread evenly over the SIMDs and the second workgroup does not fit, 16 132; 18-600-500-6 with 8 275, with 16 219)
+  const int most = R != 16 || STAGED ? 8 : lds > SNAP_HALF ? 16 : BITS == 4 ? 12 : 8;
   hipLaunchKernelGGL(kernel, dim3(p.G, (tiles + per - 1) / per), dim3(waves_for(nd, MT, most) * 64), lds, st, nd, m, p);
   return hipGetLastError();
 }
