@@ -1423,14 +1423,11 @@ static hipError_t router_run(const SnapMixture &p, int S, int A, hipStream_t st)
   return hipGetLastError();
 }
 template <int BITS, int KM>
-static hipError_t row_run(const SnapDesc &nd, const SnapMixture &p, const SnapLds &m, SnapRow at, int lds, hipStream_t st) {
+static hipError_t row_run(const SnapDesc &nd, const SnapMixture &p, const SnapLds &m, SnapRow at, int waves, int lds, hipStream_t st) {
   static LdsConfig cfg;
   const auto kernel = snap_row_kernel<BITS, 2, KM>;
   hipError_t e = ddrl_set_lds(kernel, lds, cfg);
   if (e != hipSuccess) return e;
-  int waves = p.k * at.waves;
-  const int route = KM ? (p.G + 63) / 64 : 1;               // a thread an agent
-  if (waves < route) waves = route > 16 ? 16 : route;
   hipLaunchKernelGGL(kernel, dim3(p.n), dim3(waves * 64), lds, st, nd, m, p, at);
   return hipGetLastError();
 }
@@ -1496,36 +1493,55 @@ static hipError_t sort_run(const int *idx, int total, int G, int *sorted, int *s
 static hipError_t router_launch(const SnapMixture &p, int S, int A, hipStream_t st) {
   return p.k == 1 ? router_run<1>(p, S, A, st) : p.k == 2 ? router_run<2>(p, S, A, st) : p.k <= 4 ? router_run<4>(p, S, A, st) : router_run<8>(p, S, A, st);
 }
+// A workgroup a row as long as the rows are at most two rounds of what the chip holds at once, 4 waves a SIMD: a round is 8 to 12 us,
+// the three launches of many places some 20 (top 2: 500 rows of 256 agents 45-64-64-17 in 4 bits 10.7 us, in three launches
+// 23.3; 2000 rows, two rounds, 23.5 and 26.7; 4000 rows 40.7 and 31.0; in 32 bits, one workgroup a CU, 500 rows 19.1 and
+// 23.5, 1000 rows 34 and 25; 16 agents of 18-20-6, 4000 rows 16.8 and 21.5).
+static int row_waves(const SnapMixture &p, const SnapRow &at, bool route) {
+  const int own = p.k * at.waves, agents = route ? (p.G + 63) / 64 : 1;          // (a thread an agent)
+  return own >= agents ? own : agents > 16 ? 16 : agents;
+}
 template <int BITS>
-static hipError_t mixture_few(const SnapDesc &nd, const SnapMixture &p, hipStream_t st) {
-  const int S = nd.lay[0].in, A = nd.A;
+static bool mixture_rows(const SnapDesc &nd, const SnapMixture &p, hipStream_t st, hipError_t &e) {
+  const int S = nd.lay[0].in;
   SnapLds m;
   SnapRow at;
-  const int lds = row_lds<BITS>(nd, p.k, m, at);
-  const bool together = lds <= SNAP_LDS - 1024;
-  if (together && (long long)p.G * S <= SNAP_ROUTE) return p.k <= 4 ? row_run<BITS, 4>(nd, p, m, at, lds, st) : row_run<BITS, 8>(nd, p, m, at, lds, st);
-  hipError_t e = router_launch(p, S, A, st);
+  const int lds = row_lds<BITS>(nd, p.k, m, at), most = SNAP_LDS - 1024;
+  if (lds > most) return false;
+  const bool route = (long long)p.G * S <= SNAP_ROUTE;
+  const int waves = row_waves(p, at, route), by_lds = SNAP_LDS / (lds + 64), at_once = 16 / waves < by_lds ? 16 / waves : by_lds;
+  if (p.n > 2 * 256 * at_once) return false;
+  if (!route && (e = router_launch(p, S, nd.A, st)) != hipSuccess) return true;
+  e = !route ? row_run<BITS, 0>(nd, p, m, at, waves, lds, st) : p.k <= 4 ? row_run<BITS, 4>(nd, p, m, at, waves, lds, st) : row_run<BITS, 8>(nd, p, m, at, waves, lds, st);
+  return true;
+}
+template <int BITS>
+static hipError_t mixture_places(const SnapDesc &nd, const SnapMixture &p, hipStream_t st) {
+  const hipError_t e = router_launch(p, nd.lay[0].in, nd.A, st);
   if (e != hipSuccess) return e;
-  if (together) return row_run<BITS, 0>(nd, p, m, at, lds, st);
   return fits<BITS, 1, 1, true>(nd, SNAP_HALF) ? place_run<BITS, 2, true>(nd, p, st) : place_run<BITS, 2, false>(nd, p, st);
 }
-extern "C" hipError_t snap_mixture_launch(const SnapDesc *nd, const SnapMixture *p, hipStream_t st) {
-  const int total = p->n * p->k, left = SNAP_LDS - SNAP_STATIC_LDS;
-  if (total <= SNAP_FEW) return nd->bits == 4 ? mixture_few<4>(*nd, *p, st) : mixture_few<32>(*nd, *p, st);
-  hipError_t e = router_launch(*p, nd->lay[0].in, nd->A, st);
-  if (e != hipSuccess) return e;
-  if ((e = sort_run(p->idx, total, p->G, p->sorted, p->start, st)) != hipSuccess) return e;
+extern "C" hipError_t snap_mixture_launch(const SnapDesc *nd, const SnapMixture *q, hipStream_t st) {
+  SnapMixture p = *q;
+  const int total = p.n * p.k, left = SNAP_LDS - SNAP_STATIC_LDS;
+  hipError_t e = hipSuccess;
+  if (nd->bits == 4 ? mixture_rows<4>(*nd, p, st, e) : mixture_rows<32>(*nd, p, st, e)) return e;
+  // (64 agents of 18-400-300-6 in 32 bits, top 2: 128 rows by place 28.4 us, by net 32.8; 250 rows 45.8 and 33.2)
+  if (total <= SNAP_FEW) return nd->bits == 4 ? mixture_places<4>(*nd, p, st) : mixture_places<32>(*nd, p, st);
+  p.chunks = 1;                                             // (the router picks)
+  if ((e = router_launch(p, nd->lay[0].in, nd->A, st)) != hipSuccess) return e;
+  if ((e = sort_run(p.idx, total, p.G, p.sorted, p.start, st)) != hipSuccess) return e;
   // From memory to registers, not staged (16 agents of 18-100-100-6, 1024 rows, 32 bits: 20.7 us, staged 25.3; 256 of 45-64-64-17,
   // 4096 rows: the same).  Very many places of nets that leave two workgroups a CU go in tiles of 32 rows (256 agents of 45-64-64-17,
   // 16384 rows: 93 us, in tiles of 16 109; 4096 rows 34.0 and 35.9; 2048 rows 28.1 and 26.1; 64 of 18-400-300-6, 4096 rows 109 and 103).
   const bool many = total >= 8192;
   if (nd->bits == 4) {
-    if (many && fits<4, 16, 2, false>(*nd, SNAP_HALF)) return experts_run<4, 16, 2, 1>(*nd, *p, st);
-    if (fits<4, 16, 1, false>(*nd, left)) return experts_run<4, 16, 1, 1>(*nd, *p, st);
-    return experts_run<4, 4, 1, 1>(*nd, *p, st);
+    if (many && fits<4, 16, 2, false>(*nd, SNAP_HALF)) return experts_run<4, 16, 2, 1>(*nd, p, st);
+    if (fits<4, 16, 1, false>(*nd, left)) return experts_run<4, 16, 1, 1>(*nd, p, st);
+    return experts_run<4, 4, 1, 1>(*nd, p, st);
   }
-  if (many && fits<32, 16, 2, false>(*nd, SNAP_HALF)) return experts_run<32, 16, 2, 1>(*nd, *p, st);
-  return experts_run<32, 16, 1, 1>(*nd, *p, st);                        // (fits whatever the net: 128 KiB at most)
+  if (many && fits<32, 16, 2, false>(*nd, SNAP_HALF)) return experts_run<32, 16, 2, 1>(*nd, p, st);
+  return experts_run<32, 16, 1, 1>(*nd, p, st);                        // (fits whatever the net: 128 KiB at most)
 }
 
 template <int KM>

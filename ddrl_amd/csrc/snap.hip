@@ -38,7 +38,7 @@ MixSpace mix_space(const ddrl_snap *s, int n, int k) {
   w.prob = w.idx + up16(places * 4);
   w.y = w.prob + up16(places * 4);
   w.ckey = w.y + up16(places * s->nd.A * 4);
-  w.chunks = snap_chunks(s->G, n, k);
+  w.chunks = snap_chunks(s->G, n);
   const size_t lists = w.chunks > 1 ? places * w.chunks : 0;
   w.cidx = w.ckey + up16(lists * 8);
   w.sorted = w.cidx + up16(lists * 4);
@@ -64,8 +64,8 @@ GradSpace grad_space(const ddrl_snap *s, int n, int k) {
 int check_mix_shape(const ddrl_snap *s, int n, int k) {
   if (n < 0 || k < 1 || k > DDRL_SNAP_MAX_TOP_K || k > s->G)
     return ddrl_fail(DDRL_EINVAL, "n=%d, top_k=%d: n >= 0 and 1 <= top_k <= min(%d, %d agents)", n, k, DDRL_SNAP_MAX_TOP_K, s->G);
-  if ((int64_t)n * k >= SNAP_SORT_FROM / 4 && s->G > SNAP_SORT_MAX_G)
-    return ddrl_fail(DDRL_EINVAL, "n * top_k = %lld with %d agents: %d or more places are served for up to %d agents", (long long)n * k, s->G, SNAP_SORT_FROM / 4, SNAP_SORT_MAX_G);
+  if ((int64_t)n * k >= SNAP_FEW && s->G > SNAP_SORT_MAX_G)
+    return ddrl_fail(DDRL_EINVAL, "n * top_k = %lld with %d agents: %d or more places are served for up to %d agents", (long long)n * k, s->G, SNAP_FEW, SNAP_SORT_MAX_G);
   if ((int64_t)n * k > (1 << 28)) return ddrl_fail(DDRL_EINVAL, "n * top_k = %lld over %d", (long long)n * k, 1 << 28);
   return DDRL_OK;
 }

@@ -8,8 +8,9 @@
 #define SNAP_MAXW 1024         // widest layer, as DDRL_WIDE_MAXW
 #define SNAP_MAXK 8            // DDRL_SNAP_MAX_TOP_K
 #define SNAP_LDS (160 * 1024)  // a CU's LDS
-#define SNAP_FEW 256           // places (rows x top_k) up to which a mixture gives every row, or every place, a workgroup of its own
+#define SNAP_FEW 256           // places (rows x top_k) up to which a mixture of large nets gives every place a workgroup of its own
 #define SNAP_CHUNK 256         // agents a router workgroup looks at when there are few rows
+#define SNAP_CHUNK_ROWS 4096   // rows up to which a row's agents are spread over several
 
 // An agent's net is one image of `stride` bytes: its layers one after the other, a layer a row of records, one for 16 outputs
 // (a "strip"), made for a matrix instruction whose A operand is 16 outputs by one k-step of inputs, so that a wave's load is one
@@ -56,10 +57,11 @@ __host__ __device__ inline unsigned snap_code_off(int steps, int step, int lane)
 // where the scale of (output r of a strip, step) lies in a record
 __host__ __device__ inline unsigned snap_scale_off(int code, int step, int r) { return (unsigned)code + (step >> 2) * 64 + r * 4 + (step & 3); }
 
-// how many workgroups share a row's agents: with few rows as many as there are SNAP_CHUNKs, up to 16 (the lists are merged by
-// those who answer the places), else one
-static inline int snap_chunks(int G, int n, int k) {
-  if ((long long)n * k > SNAP_FEW) return 1;
+// how many workgroups of the router share a row's agents, where those who answer the rows or places merge the lists: as many as
+// there are SNAP_CHUNKs, up to 16 (top 2: 2000 agents of 64-400-300-6, 4 rows 23.4 us, by one workgroup 48.8; 1024 of 128-64-64-6,
+// 500 rows 19.8 and 37.8, 2000 rows 38.4 and 45.5)
+static inline int snap_chunks(int G, int n) {
+  if (n > SNAP_CHUNK_ROWS) return 1;
   const int c = (G + SNAP_CHUNK - 1) / SNAP_CHUNK;
   return c > 16 ? 16 : c;
 }
@@ -98,10 +100,13 @@ struct SnapGrad {
   int *done;                          // [G] those that are through
   int piece;                          // blocks of one of them
 };
-#define SNAP_SORT_FROM 1024            // places from which the gradient sorts them first
+// places from which the gradient sorts them first (16 agents of 18 inputs: 400 places 7.7 us, sorted 8.0; 1000 places 13.9 and 8.8;
+// 1024 of 45: 6.4 and 8.1, 9.7 and 8.6)
+#define SNAP_SORT_FROM 512
 #define SNAP_SORT_MAX_G 16383          // the sort keeps a counter a net in LDS
 static inline int snap_blocks(int n, int k) { return (int)(((long long)n * k + 1023) / 1024); }
-// how many workgroups an agent: a router prefers some agents, and the places of one are what a pass waits for
+// how many workgroups an agent: a router prefers some agents, and the places of one are what a pass waits for (5 agents, 3868
+// places 12.9 us, one workgroup each 21.6; 256 agents, 16000 places 12.9 and 13.5)
 static inline int snap_grad_pieces(int G, int n, int k) {
   const int b = snap_blocks(n, k);
   int p = (1024 + G - 1) / G;

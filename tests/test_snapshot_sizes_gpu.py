@@ -230,6 +230,34 @@ def test_too_many_rows_are_refused():
             s.mixture_grad_workspace(n, 1)
 
 
+@pytest.mark.parametrize("bits, dims, g, n, k", [(4, (18, 20, 6), 10, 4096, 2), (4, (18, 20, 6), 10, 4097, 2), (32, (18, 100, 100, 6), 9, 512, 2), (32, (18, 100, 100, 6), 9, 513, 2),
+                                                 (4, (18, 64, 64, 6), 64, 512, 8), (4, (18, 64, 64, 6), 64, 513, 8), (4, (130, 40, 6), 800, 600, 2), (4, (18, 33, 5), 1024, 512, 1)])
+def test_rows_where_the_mixture_changes_its_way(bits, dims, g, n, k):
+    rng = np.random.RandomState(g)
+    s, layers = one_net(rng, g, dims, bits)
+    x = rng.uniform(-1, 1, (n, dims[0])).astype(np.float32)
+    rw, rb = rng.standard_normal((g, dims[0])).astype(np.float32), rng.standard_normal(g).astype(np.float32)
+    allowed = rng.uniform(size=(n, g)) < 0.7
+    allowed[::7] = False
+    allowed[1::7] = False
+    allowed[1::7, g // 2] = True
+    out, idx, prob, y = ask_mixture(s, x, rw, rb, k, allowed)
+    logits = np.where(allowed, x.astype(np.float64) @ rw.astype(np.float64).T + rb, -np.inf)
+    wi = np.argsort(-logits, 1, kind="stable")[:, :k]
+    l = np.take_along_axis(logits, wi, 1)
+    have = np.isfinite(l)
+    p = np.where(have, np.exp(l - np.where(have[:, :1], l[:, :1], 0)), 0)
+    p = p / np.maximum(p.sum(1, keepdims=True), 1e-300)
+    assert np.array_equal(idx, np.where(have, wi, -1)) and np.abs(prob - p).max() <= 200 * sc.U
+    v, e = sc.forward([(w[:1], b[:1]) for w, b in layers], x[None], HIDDEN, LAST)       # all nets are one
+    v, e = np.where(have[..., None], v[0][:, None], 0), np.where(have[..., None], e[0][:, None], 0)
+    within(y, v, e + 1e-37)
+    pe = (8 + 176 + k + 1) * sc.U                                 # as in snapshot_common.mixture
+    within(out, (p[..., None] * v).sum(1), (p[..., None] * (e + (pe + (k + 1) * sc.U) * (np.abs(v) + e))).sum(1) + 1e-37)
+    again = ask_mixture(s, x, rw, rb, k, allowed)
+    assert all(np.array_equal(a, b) for a, b in zip((out, idx, prob, y), again))
+
+
 # ---- graphs and streams of each way of working ---------------------------------------------------------------------------
 
 @pytest.mark.parametrize("bits, dims, g, n, k", [(4, (18, 400, 300, 6), 300, 6, 8), (32, (18, 400, 300, 6), 7, 10, 2), (32, (97, 40, 6), 1100, 5, 3), (4, (18, 33, 6), 9, 4200, 2),
