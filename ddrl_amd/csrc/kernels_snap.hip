@@ -1495,24 +1495,28 @@ static hipError_t router_launch(const SnapMixture &p, int S, int A, hipStream_t 
 }
 // A workgroup a row as long as the rows are at most two rounds of what the chip holds at once, 4 waves a SIMD: a round is 8 to 12 us,
 // the three launches of many places some 20 (top 2: 500 rows of 256 agents 45-64-64-17 in 4 bits 10.7 us, in three launches
-// 23.3; 2000 rows, two rounds, 23.5 and 26.7; 4000 rows 40.7 and 31.0; in 32 bits, one workgroup a CU, 500 rows 19.1 and
-// 23.5, 1000 rows 34 and 25; 16 agents of 18-20-6, 4000 rows 16.8 and 21.5).
-static int row_waves(const SnapMixture &p, const SnapRow &at, bool route) {
-  const int own = p.k * at.waves, agents = route ? (p.G + 63) / 64 : 1;          // (a thread an agent)
-  return own >= agents ? own : agents > 16 ? 16 : agents;
+// 23.3; 2000 rows, two rounds, 20.6 and 26.7; 4000 rows 40.7 and 31.0; in 32 bits, one workgroup a CU, 500 rows 19 to 21 and
+// 23.5, 1000 rows 34 and 25; 16 agents of 18-20-6, 4000 rows 15.5 and 21.5).
+// It is its own router as long as that is one round (the same 256 agents: 1000 rows 14.3 us, with a router of its own 16.9; 2000
+// rows 24.1 and 20.6; 1024 agents, whose router takes 16 waves: 200 rows 14.2 and 19.1, 500 rows 23.7 and 16.2).
+static int rows_at_once(int waves, int lds) {
+  const int by_waves = 16 / waves, by_lds = SNAP_LDS / (lds + 64);
+  return 256 * (by_waves < by_lds ? by_waves : by_lds);
 }
 template <int BITS>
 static bool mixture_rows(const SnapDesc &nd, const SnapMixture &p, hipStream_t st, hipError_t &e) {
   const int S = nd.lay[0].in;
   SnapLds m;
   SnapRow at;
-  const int lds = row_lds<BITS>(nd, p.k, m, at), most = SNAP_LDS - 1024;
-  if (lds > most) return false;
-  const bool route = (long long)p.G * S <= SNAP_ROUTE;
-  const int waves = row_waves(p, at, route), by_lds = SNAP_LDS / (lds + 64), at_once = 16 / waves < by_lds ? 16 / waves : by_lds;
-  if (p.n > 2 * 256 * at_once) return false;
-  if (!route && (e = router_launch(p, S, nd.A, st)) != hipSuccess) return true;
-  e = !route ? row_run<BITS, 0>(nd, p, m, at, waves, lds, st) : p.k <= 4 ? row_run<BITS, 4>(nd, p, m, at, waves, lds, st) : row_run<BITS, 8>(nd, p, m, at, waves, lds, st);
+  const int lds = row_lds<BITS>(nd, p.k, m, at);
+  if (lds > SNAP_LDS - 1024) return false;
+  const int own = p.k * at.waves, agents = p.G > 1024 ? 16 : (p.G + 63) / 64, all = own > agents ? own : agents;    // (a thread an agent)
+  if ((long long)p.G * S <= SNAP_ROUTE && p.n <= rows_at_once(all, lds)) {
+    e = p.k <= 4 ? row_run<BITS, 4>(nd, p, m, at, all, lds, st) : row_run<BITS, 8>(nd, p, m, at, all, lds, st);
+    return true;
+  }
+  if (p.n > 2 * rows_at_once(own, lds)) return false;
+  if ((e = router_launch(p, S, nd.A, st)) == hipSuccess) e = row_run<BITS, 0>(nd, p, m, at, own, lds, st);
   return true;
 }
 template <int BITS>
