@@ -151,8 +151,9 @@ extern "C" hipError_t snap_load_launch(const SnapDesc *nd, char *img, const Snap
 // bank conflict, every one of a block of steps at a constant distance from the first.  Instructions, not bytes, bound a net
 // of many rows, so what is left of addresses is a scalar or such a constant (1024 agents of 18-400-300-6, 64 rows: 95 us, 530
 // TFLOP/s of the three bf16 products; 147 us with 7 vector instructions a product and row-major inputs.  A wave of several strips or
-// tiles at once shares more, and leaves waves idle where a layer ends: 110 to 196 us).  One row is bound by its net's bytes
-// and by the layers' latency, some 3000 cycles each (84 MB of them: 21.4 us, 3.9 TB/s).
+// tiles at once shares more, and leaves waves idle where a layer ends: 110 to 196 us).  One row is bound by
+// the layers' latency, some 3000 cycles each, and by decoding and the sums' ends, half of a SIMD's cycles, before its net's bytes
+// (84 MB of them: 21.4 us, 3.9 TB/s).
 // ------------------------------------------------------------------------------------------------------------------------
 struct SnapLds { int second, image; };          // the inputs of layers 0, 2 lie in the first LDS buffer, those of 1, 3 in the second; behind them the image, where it is staged
 
