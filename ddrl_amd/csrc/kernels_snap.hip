@@ -1407,6 +1407,9 @@ extern "C" hipError_t snap_forward_launch(const SnapDesc *nd, const SnapForward 
   return fits<32, 1, 1, true>(*nd, SNAP_HALF) ? forward_run<32, 1, 2, true>(*nd, *p, st) : forward_run<32, 1, 2, false>(*nd, *p, st);
 }
 
+// A launch has at most 2^32 - 1 threads along x: rows (places) that one launch of the router (of the gradient's first kernel) takes,
+// of 32 (16) threads each at most
+#define SNAP_AT_ONCE (1 << 26)
 template <int KM>
 static hipError_t router_run(const SnapMixture &p, int S, int A, hipStream_t st) {
   const int ld = ddrl_roundup(S, 64) + 4;
@@ -1420,8 +1423,18 @@ static hipError_t router_run(const SnapMixture &p, int S, int A, hipStream_t st)
   static LdsConfig cfg;
   hipError_t e = ddrl_set_lds(snap_router_kernel<KM>, lds, cfg);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(snap_router_kernel<KM>, dim3((p.n + 15) / 16, p.chunks), dim3(waves * 64), lds, st, p, S, A, ld);
-  return hipGetLastError();
+  for (int64_t t = 0; t < p.n && e == hipSuccess; t += SNAP_AT_ONCE) {      // (more rows than one launch takes: never in chunks)
+    SnapMixture part = p;
+    part.n = (int)(p.n - t < SNAP_AT_ONCE ? p.n - t : SNAP_AT_ONCE);
+    part.x += t * p.x_row;
+    if (p.allowed) part.allowed += t * p.a_row;
+    part.out += t * p.out_row;
+    part.idx += t * p.k; part.prob += t * p.k; part.y += t * p.k * A;
+    part.count += t;
+    hipLaunchKernelGGL(snap_router_kernel<KM>, dim3((part.n + 15) / 16, p.chunks), dim3(waves * 64), lds, st, part, S, A, ld);
+    e = hipGetLastError();
+  }
+  return e;
 }
 template <int BITS, int KM>
 static hipError_t row_run(const SnapDesc &nd, const SnapMixture &p, const SnapLds &m, SnapRow at, int waves, int lds, hipStream_t st) {
@@ -1559,8 +1572,22 @@ static hipError_t grad_first_run(const SnapGrad &p, hipStream_t st) {
   static LdsConfig cfg;
   hipError_t e = ddrl_set_lds(snap_grad_first_kernel<KM>, lds, cfg);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(snap_grad_first_kernel<KM>, dim3(p.blocks + (p.n * p.k + 63) / 64), dim3(1024), lds, st, p, sort_bits(p.G));
-  return hipGetLastError();
+  // the first launch sorts all places and takes the first of the dlogits, the others (over 2^26 places) go on; 64 rows are whole workgroups
+  const int64_t rows = SNAP_AT_ONCE / p.k / 64 * 64;
+  for (int64_t t = 0; t < p.n && e == hipSuccess; t += rows) {
+    const int64_t now = p.n - t < rows ? p.n - t : rows;
+    SnapGrad part = p;
+    if (t) {
+      part.blocks = 0;
+      part.n = (int)now;
+      part.idx += t * p.k; part.prob += t * p.k; part.y += t * p.k * p.A; part.dout += t * p.dout_row;
+      if (p.dy) part.dy += t * p.k * p.A;
+      part.dlogit += t * p.k;
+    }
+    hipLaunchKernelGGL(snap_grad_first_kernel<KM>, dim3((unsigned)(part.blocks + (now * p.k + 63) / 64)), dim3(1024), lds, st, part, sort_bits(p.G));
+    e = hipGetLastError();
+  }
+  return e;
 }
 extern "C" hipError_t snap_grad_launch(const SnapGrad *q, int pieces, hipStream_t st) {
   SnapGrad p = *q;

@@ -356,3 +356,41 @@ def test_rows_that_overlap_in_memory():
     x = np.lib.stride_tricks.sliding_window_view(series, 18)
     want, bound = sc.forward(layers, np.broadcast_to(x, (3,) + x.shape), HIDDEN, LAST)
     within(out.cpu().numpy(), want, bound)
+
+
+def test_as_many_rows_as_are_served():
+    """2^28 places, in the mixture and in the gradient: more threads than one launch takes.  Small whole numbers, so that every
+    answer and every sum of 64 bits is exact."""
+    import ddrl_amd
+    n = 2 ** 28
+    s = ddrl_amd.PolicySnapshot.shaped(2, 1, 1, [], 0, 0, bits=32)
+    flat = dev(np.array([[3, 1], [-2, 5]], np.float32))               # weight, bias
+    torch.cuda.synchronize()
+    s.load_flat_dev(flat.data_ptr(), 2)
+    gen = torch.Generator(DEV).manual_seed(1)
+    small = lambda: torch.randint(-3, 4, (n,), generator=gen, device=DEV, dtype=torch.int8).float()
+    x, rw, rb = small(), dev(np.array([[1], [-1]], np.float32)), dev(np.array([1, 0], np.float32))
+    out, prob, y = (torch.full((n,), 77.0, device=DEV) for _ in range(3))
+    idx = torch.full((n,), 77, dtype=torch.int32, device=DEV)
+    ws = torch.empty(s.mixture_workspace(n, 1), dtype=torch.uint8, device=DEV)
+    q = torch.cuda.current_stream().cuda_stream
+    s.mixture_dev(s.mixture_args(n, 1, x.data_ptr(), rw.data_ptr(), out.data_ptr(), router_b=rb.data_ptr(), idx=idx.data_ptr(), prob=prob.data_ptr(), y=y.data_ptr(),
+                                 workspace=ws.data_ptr(), workspace_bytes=ws.numel(), stream=q))
+    torch.cuda.synchronize()
+    first = x + 1 >= -x
+    want = torch.where(first, 3 * x + 1, -2 * x + 5)
+    assert bool((idx == torch.where(first, 0, 1)).all()) and bool((prob == 1).all())
+    assert bool((y == want).all()) and bool((out == want).all())
+    del ws, out, want, first
+    dout = small()
+    prob.fill_(0.5)
+    dw, db, dy = torch.zeros(2, device=DEV), torch.zeros(2, device=DEV), torch.full((n,), 77.0, device=DEV)
+    ws = torch.empty(s.mixture_grad_workspace(n, 1), dtype=torch.uint8, device=DEV)
+    s.mixture_grad_dev(s.mixture_grad_args(n, 1, x.data_ptr(), idx.data_ptr(), prob.data_ptr(), y.data_ptr(), dout.data_ptr(), dw.data_ptr(), db.data_ptr(), dy.data_ptr(),
+                                           workspace=ws.data_ptr(), workspace_bytes=ws.numel(), stream=q))
+    torch.cuda.synchronize()
+    assert bool((dy == 0.5 * dout).all())
+    for e in range(2):
+        dl = torch.where(idx == e, 0.25 * (y * dout), 0)              # .5 (s - .5 s)
+        assert dw[e].item() == np.float32((dl * x).sum(dtype=torch.float64).item())
+        assert db[e].item() == np.float32(dl.sum(dtype=torch.float64).item())
