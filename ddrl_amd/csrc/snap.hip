@@ -89,7 +89,7 @@ extern "C" int ddrl_snap_create(int n_agents, int in_dim, int out_dim, const int
                                 int output_layer_type, int bits, int device, ddrl_snap_t **out) {
   if (!out || (n_hidden > 0 && !hidden)) return ddrl_fail(DDRL_EINVAL, "NULL argument");
   *out = nullptr;
-  if (n_agents < 1) return ddrl_fail(DDRL_EINVAL, "n_agents < 1");
+  if (n_agents < 1 || n_agents > SNAP_MAX_G) return ddrl_fail(DDRL_EINVAL, "n_agents=%d outside 1..%d", n_agents, SNAP_MAX_G);
   if (n_hidden < 0 || n_hidden > DDRL_MAX_HIDDEN) return ddrl_fail(DDRL_EINVAL, "n_hidden=%d outside 0..%d", n_hidden, DDRL_MAX_HIDDEN);
   if (in_dim < 1 || in_dim > SNAP_MAXW || out_dim < 1 || out_dim > SNAP_MAXW)
     return ddrl_fail(DDRL_EINVAL, "in_dim=%d / out_dim=%d outside 1..%d", in_dim, out_dim, SNAP_MAXW);

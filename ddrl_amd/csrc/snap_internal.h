@@ -7,6 +7,7 @@
 #define SNAP_MAXL 4            // InnerProducts of a net (up to three hidden layers)
 #define SNAP_MAXW 1024         // widest layer, as DDRL_WIDE_MAXW
 #define SNAP_MAXK 8            // DDRL_SNAP_MAX_TOP_K
+#define SNAP_MAX_G 4194303     // agents: a launch has at most 2^32 - 1 threads along x, a workgroup of up to 1024 for each agent
 #define SNAP_LDS (160 * 1024)  // a CU's LDS
 #define SNAP_FEW 256           // places (rows x top_k) up to which a mixture of large nets gives every place a workgroup of its own
 #define SNAP_CHUNK 256         // agents a router workgroup looks at when there are few rows

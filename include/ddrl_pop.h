@@ -576,8 +576,8 @@ int ddrl_sim_run_episode(ddrl_sim_t *s, int learning, long lepisode, long tepiso
 typedef struct ddrl_snap ddrl_snap_t;
 #define DDRL_SNAP_MAX_TOP_K 8
 
-/* an empty snapshot (zero weights) for nets in_dim - hidden[0] - .. - out_dim: dimensions 1..1024, 0..3 hidden layers;
- * hidden_layer_type 0..3, output_layer_type 0..3 (0 linear, 1 leaky-ReLU(0.01), 2 tanh, 3 ReLU); bits 32 or 4 */
+/* an empty snapshot (zero weights) of 1..4194303 agents for nets in_dim - hidden[0] - .. - out_dim: dimensions 1..1024, 0..3 hidden
+ * layers; hidden_layer_type 0..3, output_layer_type 0..3 (0 linear, 1 leaky-ReLU(0.01), 2 tanh, 3 ReLU); bits 32 or 4 */
 int ddrl_snap_create(int n_agents, int in_dim, int out_dim, const int *hidden, int n_hidden, int hidden_layer_type,
                      int output_layer_type, int bits, int device, ddrl_snap_t **out);
 /* the same with the dimensions, activations and GPU of a population's net, loaded from it */

@@ -77,3 +77,12 @@ def test_definition_of_four_bits():
         assert np.all(np.abs(q - v) <= gap * s[:, None] + 1e-300)
     ties = np.array([[.25, .75, 1.25, 1.75, 2.5, 3.5, 5., 6., -.25, -.75, -5., -2.5]], np.float32)
     assert np.array_equal(sc.round4(ties)[0], [0, 1, 1, 2, 2, 4, 4, 6, 0, -1, -4, -2])
+
+
+@pytest.mark.parametrize("n_agents", [2 ** 22, 2 ** 24, 2 ** 31 - 1])
+def test_more_agents_than_a_launch_takes_are_refused(n_agents):
+    """a workgroup an agent, 1024 threads at most, 2^32 - 1 threads in all"""
+    import ddrl_amd
+    with pytest.raises(ddrl_amd.DdrlError) as e:
+        _create(n_agents=n_agents)
+    assert e.value.code == -1 and "n_agents" in str(e.value)

@@ -394,3 +394,30 @@ def test_as_many_rows_as_are_served():
         dl = torch.where(idx == e, 0.25 * (y * dout), 0)              # .5 (s - .5 s)
         assert dw[e].item() == np.float32((dl * x).sum(dtype=torch.float64).item())
         assert db[e].item() == np.float32(dl.sum(dtype=torch.float64).item())
+
+
+def test_as_many_agents_as_there_may_be():
+    """2^22 - 1 agents, asked in every way"""
+    import ddrl_amd
+    g, k = 2 ** 22 - 1, 2
+    s = ddrl_amd.PolicySnapshot.shaped(g, 1, 1, [], 0, 0, bits=4)
+    gen = torch.Generator(DEV).manual_seed(2)
+    flat = torch.stack((torch.tensor([.5, 1., 1.5, 2., 3., 4., 6.], device=DEV)[torch.randint(0, 7, (g,), generator=gen, device=DEV)],
+                        torch.randint(-9, 10, (g,), generator=gen, device=DEV).float()), 1).contiguous()
+    torch.cuda.synchronize()
+    s.load_flat_dev(flat.data_ptr(), 2)
+    x = torch.randint(-3, 4, (g, 1, 1), generator=gen, device=DEV, dtype=torch.int8).float()
+    out = torch.full((g, 1, 1), 77.0, device=DEV)
+    q = torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    s.forward_dev(s.forward_args(1, x.data_ptr(), out.data_ptr(), stream=q))
+    assert bool((out[:, 0, 0] == flat[:, 0] * x[:, 0, 0] + flat[:, 1]).all())
+    rw = torch.zeros(g, 1, device=DEV)
+    rw[[5, g - 1], 0] = torch.tensor([1., 2.], device=DEV)
+    one = np.ones((1, 1), np.float32)
+    got, idx, prob, y = ask_mixture(s, one, rw.cpu().numpy(), None, k)
+    assert idx.tolist() == [[g - 1, 5]] and np.array_equal(y[0, :, 0], flat[[g - 1, 5]].sum(1).cpu().numpy())
+    dw, db, _ = ask_grad(s, one, idx, np.array([[.5, .5]]), np.array([[[4.], [2.]]]), one)
+    want = np.zeros((g, 1), np.float32)
+    want[[g - 1, 5], 0] = .5, -.5                                     # .5 (4 - 3), .5 (2 - 3)
+    assert np.array_equal(dw, want) and np.array_equal(db, want[:, 0])
