@@ -250,9 +250,9 @@ static int forward_on(ddrl_snap *s, const ddrl_snap_forward_args *a, hipStream_t
   p.G = s->G; p.n = a->n; p.per = 0; p.img = s->img;
   p.x = a->x; p.out = a->out; p.mask = a->mask;
   p.x_row = a->x_row == -1 ? S : a->x_row;
-  p.x_agent = a->x_agent == -1 ? n * p.x_row : a->x_agent;
+  p.x_agent = a->x_agent != -1 ? a->x_agent : p.x_row ? n * p.x_row : S;           // (x_row 0: an agent has one row)
   p.out_row = a->out_row == -1 ? A : a->out_row;
-  p.out_agent = a->out_agent == -1 ? n * p.out_row : a->out_agent;
+  p.out_agent = a->out_agent != -1 ? a->out_agent : p.out_row ? n * p.out_row : A;
   if (p.x_row < 0 || p.x_agent < 0) return ddrl_fail(DDRL_EINVAL, "negative stride of x");
   // rows of an agent one after the other and agents apart, or the agents of a row one after the other and rows apart
   const bool rows_in = (n == 1 || p.out_row >= A) && (G == 1 || p.out_agent >= (n - 1) * p.out_row + A);

@@ -599,7 +599,8 @@ int ddrl_snap_get_weights(ddrl_snap_t *s, double *flat);
 typedef struct {
   int n;                                   /* rows per agent, 0..2^28 */
   const float *x;
-  int64_t x_agent, x_row;                  /* x_agent 0: all agents read the same n rows; x_row 0: an agent's rows are one row */
+  int64_t x_agent, x_row;                  /* x_agent 0: all agents read the same n rows; x_row 0: an agent's rows are one row
+                                              (x_agent -1: n * x_row, where that is 0 in_dim; out_agent likewise) */
   float *out;
   int64_t out_agent, out_row;
   const uint8_t *mask;                     /* [n_agents] or NULL; an agent with mask 0 is skipped, its rows of out stay as they were */

@@ -421,3 +421,26 @@ def test_as_many_agents_as_there_may_be():
     want = np.zeros((g, 1), np.float32)
     want[[g - 1, 5], 0] = .5, -.5                                     # .5 (4 - 3), .5 (2 - 3)
     assert np.array_equal(dw, want) and np.array_equal(db, want[:, 0])
+
+
+@pytest.mark.parametrize("bits", [32, 4])
+@pytest.mark.parametrize("n", [1, 3, 20])
+def test_one_row_an_agent_packed(n, bits):
+    """x_row = 0 with the agents' rows packed: agent g reads row g; out_row = 0 for a single row likewise"""
+    dims, g = (18, 33, 5), 4
+    rng = np.random.RandomState(n)
+    flat = make_flat(rng, g, dims)
+    s = make_snap(flat, dims, bits)
+    x = rng.uniform(-1, 1, (g, 1, 18)).astype(np.float32)
+    want, bound = sc.forward(sc.stored(sc.split_flat(flat, dims), bits), np.broadcast_to(x, (g, n, 18)), HIDDEN, LAST)
+    xd, out = dev(x), torch.full((g, n, 5), 77.0, device=DEV)
+    torch.cuda.synchronize()
+    s.forward_dev(s.forward_args(n, xd.data_ptr(), out.data_ptr(), x_row=0, out_row=0 if n == 1 else None))
+    torch.cuda.synchronize()
+    within(out.cpu().numpy(), want, bound)
+    xd = dev(rng.uniform(-1, 1, (1, 18)).astype(np.float32))              # one row for all agents
+    torch.cuda.synchronize()
+    s.forward_dev(s.forward_args(n, xd.data_ptr(), out.data_ptr(), x_agent=0, x_row=0))
+    torch.cuda.synchronize()
+    want, bound = sc.forward(sc.stored(sc.split_flat(flat, dims), bits), np.broadcast_to(xd.cpu().numpy(), (g, n, 18)), HIDDEN, LAST)
+    within(out.cpu().numpy(), want, bound)
