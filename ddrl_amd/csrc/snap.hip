@@ -241,8 +241,12 @@ extern "C" int ddrl_snap_get_weights(ddrl_snap_t *s, double *flat) {
   return DDRL_OK;
 }
 
+static int check_rows(int n) {
+  if (n < 0 || n > (1 << 28)) return ddrl_fail(DDRL_EINVAL, "n=%d: 0..%d", n, 1 << 28);
+  return DDRL_OK;
+}
 static int forward_on(ddrl_snap *s, const ddrl_snap_forward_args *a, hipStream_t st) {
-  if (a->n < 0 || a->n > (1 << 28)) return ddrl_fail(DDRL_EINVAL, "n=%d: 0..%d", a->n, 1 << 28);
+  if (check_rows(a->n)) return DDRL_EINVAL;
   if (a->n == 0) return DDRL_OK;
   if (!a->x || !a->out || off4(a->x) || off4(a->out)) return ddrl_fail(DDRL_EINVAL, "x / out NULL or misaligned");
   const int64_t S = s->nd.lay[0].in, A = s->nd.A, n = a->n, G = s->G;
@@ -270,7 +274,8 @@ extern "C" int ddrl_snap_forward_dev(ddrl_snap_t *s, const ddrl_snap_forward_arg
 }
 
 extern "C" int ddrl_snap_forward(ddrl_snap_t *s, int n, const float *x, float *out) {
-  if (!s || n < 0 || (n && (!x || !out))) return ddrl_fail(DDRL_EINVAL, "bad argument");
+  if (!s || (n && (!x || !out))) return ddrl_fail(DDRL_EINVAL, "NULL argument");
+  if (check_rows(n)) return DDRL_EINVAL;
   if (n == 0) return DDRL_OK;
   ON_DEVICE(s);
   const size_t nx = (size_t)s->G * n * s->nd.lay[0].in * 4, no = (size_t)s->G * n * s->nd.A * 4;

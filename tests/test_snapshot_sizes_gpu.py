@@ -444,3 +444,13 @@ def test_one_row_an_agent_packed(n, bits):
     torch.cuda.synchronize()
     want, bound = sc.forward(sc.stored(sc.split_flat(flat, dims), bits), np.broadcast_to(xd.cpu().numpy(), (g, n, 18)), HIDDEN, LAST)
     within(out.cpu().numpy(), want, bound)
+
+
+def test_the_host_form_refuses_before_it_reads():
+    s = make_snap(make_flat(np.random.RandomState(1), 2, (3, 2)), (3, 2), 4)
+    two = np.zeros(12, np.float32)
+    for n in (-1, 2 ** 28 + 1, 2 ** 31 - 1):
+        assert s.L.ddrl_snap_forward(s.h, n, two.ctypes.data, two.ctypes.data) == -1
+        assert ("n=%d" % n).encode() in s.L.ddrl_last_error()
+        assert s.L.ddrl_snap_mixture(s.h, n, 1, two.ctypes.data, two.ctypes.data, None, None, two.ctypes.data, None, None) == -1
+    assert s.L.ddrl_snap_forward(s.h, 1, None, two.ctypes.data) == -1 and s.L.ddrl_snap_forward(s.h, 0, None, None) == 0
