@@ -720,7 +720,9 @@ template <int KM> struct Best {
     }
   }
 };
-// the softmax over the picks that 16 lanes hold
+// The softmax over the picks that 16 lanes hold.  The logits' differences are taken in fp64 and rounded once: from there on a 32-bit
+// number comes out and weighs 32-bit answers, and what the rounding, expf, the sum and the division add, (|difference| + 14) 2^-24
+// of it at most, is of the size of what the answers are off by themselves.
 __device__ __forceinline__ float pick_prob(unsigned long long mk, int mi) {
   const unsigned long long tk = (unsigned long long)(unsigned)first_of_16((int)(mk >> 32)) << 32 | (unsigned)first_of_16((int)mk);
   const float ex = mi != IDX_NONE ? expf((float)(key_logit(mk) - key_logit(tk))) : 0.f;
@@ -1160,9 +1162,12 @@ snap_experts_kernel(const SnapDesc nd_, const SnapLds m, const SnapMixture p) {
 // Few places: one launch, a workgroup per agent looks through idx itself, 256 places at once, and sums dlogit x over its own:
 // thread (u, s) over the collected places u, u + parts, .. of input s, and the parts in their order.
 // Many: a first launch takes all dlogits and, in other workgroups, sorts the places by agent; in a second one a workgroup per agent
-// sums over the places that picked it, in their order, a wave every fourth of them and a lane an input.  Few agents: several
-// workgroups each, a run of sorted blocks every one; their sums go to the workspace, and the last of them adds all, in order.
-// Sums over rows are in fp64 (an agent may be picked by every row).  Bound by launches and latency: 16 agents of 18 inputs, 9 rows,
+// sums over the places that picked it, a wave every fourth of them, a lane an input, then the waves' sums.  Few agents: several
+// workgroups each, a run of sorted blocks every one; their sums go to the workspace, and the last of them adds all.  So the order
+// of a sum hangs on the sizes, never on who came first.
+// Sums over rows are in fp64 (an agent may be picked by every row).  A dlogit is fp32: its dot products have as many terms as the
+// nets have outputs, of answers that are fp32 sums themselves, and it is off by (outputs + top_k + 4) 2^-24 of the terms' magnitudes
+// at most, once a place.  Bound by launches and latency: 16 agents of 18 inputs, 9 rows,
 // top 2: 4.1 us; 1024 of 45, 4096 rows, top 4: 5.9 and 6.3 us (sums by the workgroup of an agent over unsorted idx: 65).
 // ------------------------------------------------------------------------------------------------------------------------
 // dlogit of a place, in all of its 16 lanes (a0 = 0 .. 15), and dy; one that picked nobody: 0

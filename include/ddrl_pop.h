@@ -563,7 +563,8 @@ int ddrl_sim_run_episode(ddrl_sim_t *s, int learning, long lepisode, long tepiso
  * that 32 consecutive inputs of one output share (the last block of a row may be shorter).  Loading takes the least power
  * of two that keeps the block's largest magnitude within 6 and rounds to the nearest, halves to the even code.  A block
  * whose largest magnitude is under 2^-118 becomes zeros; an output with a weight that is not finite, or of magnitude 2^126
- * or more, answers NaN.  Biases stay in 32 bits.  Activations and sums are 32-bit in both formats.
+ * or more, answers NaN.  Biases stay in 32 bits.  Activations and sums are 32-bit in both formats (4-bit weights meet what an
+ * activation is to within 2^-133).
  *
  * A snapshot is not written by the calls that ask it, and they keep nothing in it: the _dev calls take the stream to run on
  * and, where they need one, a workspace of the caller's.  They may be captured into a HIP graph, and calls on several
@@ -638,8 +639,9 @@ int ddrl_snap_mixture(ddrl_snap_t *s, int n, int top_k, const float *x, const fl
  *     dlogit[t, j] = prob[t, j] (dout[t] . y[t, j] - sum_i prob[t, i] dout[t] . y[t, i])
  *     d_router_w[g, :] = sum over the places (t, j) with idx[t, j] = g of dlogit[t, j] x[t],   d_router_b[g] = sum of dlogit[t, j]
  *     dy[t, j] = prob[t, j] dout[t]         (dL/dy, for whoever goes on into the nets)
- * summed in the order of t: the same bits every time.  Places whose idx is outside 0..n_agents-1 add nothing and get dy = 0.
- * The gradients are written, not added to; a net nobody picked gets zeros. */
+ * dlogit in 32 bits, its sums over places in 64, in an order that the call's sizes and outputs fix (not that of t): the same
+ * call gives the same bits.  Places whose idx is outside 0..n_agents-1 add nothing and get dy = 0.  The gradients are written,
+ * not added to; a net nobody picked gets zeros. */
 typedef struct {
   int n, top_k;
   const float *x; int64_t x_row;
