@@ -46,8 +46,9 @@ __device__ __forceinline__ f32x4 act_four(int act, f32x4 x) {
 // Loading.  One wave per (agent, layer, strip): lane (r, q) walks the k-steps of output r; the four lanes of an output agree
 // on a block's largest magnitude.  With amax = m 2^e, m in [1, 2): amax <= 6 2^s for the least s = e - 2 (m <= 1.5) or e - 1,
 // so the scale comes out of the exponent field alone, and w 2^-s is exact: the codes do not depend on any rounding of the
-// machine's.  Bound by the reads of the fp32 parameters, 16 bytes a lane and a block of four steps at a time (1024 agents of
-// 18-400-300-6 to 4 bits, 530 MB: 197 us, 2.7 TB/s; a wave's blocks come one after the other).
+// machine's.  Reads 16 bytes a lane and a block of four steps at a time, and waits for them: a block is asked for when the one before
+// is encoded (1024 agents of 18-400-300-6 to 4 bits: 530 MB in, 84 MB out, 170 to 197 us, 3.1 to 3.6 TB/s; a
+// copy reaches 4.8).
 // ------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ unsigned snap_code(float v) {          // v = w / scale, |v| <= 6: nearest of the grid, halves to the even code
   const float a = fabsf(v);
@@ -148,12 +149,13 @@ extern "C" hipError_t snap_load_launch(const SnapDesc *nd, char *img, const Snap
 // end.  And with R < 16 every lane finishes ONE output of the tile (bias, activation, the three parts) instead of a few lanes
 // finishing four: with few rows that, not the product, is most of the instructions.
 // Activations lie as the B operand is read, [k-step][part][16 rows][k quarter][row] x 16 bytes: a wave's read is 1 KiB without a
-// bank conflict, every one of a block of steps at a constant distance from the first.  Instructions, not bytes, bound a net
-// of many rows, so what is left of addresses is a scalar or such a constant (1024 agents of 18-400-300-6, 64 rows: 95 us, 530
-// TFLOP/s of the three bf16 products; 147 us with 7 vector instructions a product and row-major inputs.  A wave of several strips or
-// tiles at once shares more, and leaves waves idle where a layer ends: 110 to 196 us).  One row is bound by
-// the layers' latency, some 3000 cycles each, and by decoding and the sums' ends, half of a SIMD's cycles, before its net's bytes
-// (84 MB of them: 21.4 us, 3.9 TB/s).
+// bank conflict, every one of a block of steps at a constant distance from the first.  Instructions and waits, not bytes, bound a
+// net of many rows, so what is left of addresses is a scalar or such a constant (1024 agents of 18-400-300-6, 64 rows: 94 us, 540
+// TFLOP/s of the three bf16 products, the vector units at work 60 % of the time, the matrix cores 28, a wave waiting 52; 147 us with
+// 7 vector instructions a product and row-major inputs.  A wave of several strips or tiles at once shares more, and leaves waves
+// idle where a layer ends: 110 to 196 us).  One row is bound by the layers' latency, a wave waiting 60 % of its time, and by decoding
+// and the sums' ends, half of the vector units' time, before its net's bytes (84 MB of them: 21.4 us, 3.9 TB/s, out of the last-level
+// cache; 26.0 out of memory).
 // ------------------------------------------------------------------------------------------------------------------------
 struct SnapLds { int second, image; };          // the inputs of layers 0, 2 lie in the first LDS buffer, those of 1, 3 in the second; behind them the image, where it is staged
 
