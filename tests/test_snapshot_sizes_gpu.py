@@ -454,3 +454,49 @@ def test_the_host_form_refuses_before_it_reads():
         assert ("n=%d" % n).encode() in s.L.ddrl_last_error()
         assert s.L.ddrl_snap_mixture(s.h, n, 1, two.ctypes.data, two.ctypes.data, None, None, two.ctypes.data, None, None) == -1
     assert s.L.ddrl_snap_forward(s.h, 1, None, two.ctypes.data) == -1 and s.L.ddrl_snap_forward(s.h, 0, None, None) == 0
+
+
+def test_strides_and_masks_over_several_launches():
+    """more rows than one launch of the router takes: where a later launch starts, every array's rows are the ones a small call of
+    the same rows answers; sums are exact (small whole numbers, prob = .5)"""
+    import ddrl_amd
+    n, k = 2 ** 26 + 5000, 2
+    s = ddrl_amd.PolicySnapshot.shaped(3, 1, 1, [], 0, 0, bits=32)
+    flat = dev(np.array([[3, 1], [-2, 5], [1, -4]], np.float32))
+    torch.cuda.synchronize()
+    s.load_flat_dev(flat.data_ptr(), 2)
+    gen = torch.Generator(DEV).manual_seed(3)
+    small = lambda *shape: torch.randint(-3, 4, shape, generator=gen, device=DEV, dtype=torch.int8).float()
+    x, dout = small(n, 2), small(n, 3)
+    allowed = (torch.rand(n, 4, generator=gen, device=DEV) < 0.6).to(torch.uint8)
+    rw, rb = dev(np.array([[1], [-1], [2]], np.float32)), dev(np.array([1, 0, -1], np.float32))
+    q = torch.cuda.current_stream().cuda_stream
+
+    def ask_rows(a, b):
+        m = b - a
+        out, prob, y = torch.full((m, 2), 77.0, device=DEV), torch.full((m, k), 77.0, device=DEV), torch.full((m, k), 77.0, device=DEV)
+        idx, ws = torch.full((m, k), 77, dtype=torch.int32, device=DEV), torch.empty(s.mixture_workspace(m, k), dtype=torch.uint8, device=DEV)
+        s.mixture_dev(s.mixture_args(m, k, x[a:].data_ptr() + 4, rw.data_ptr(), out.data_ptr(), router_b=rb.data_ptr(), allowed=allowed[a:].data_ptr() + 1, idx=idx.data_ptr(),
+                                     prob=prob.data_ptr(), y=y.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=ws.numel(), x_row=2, allowed_row=4, out_row=2, stream=q))
+        torch.cuda.synchronize()
+        return out, idx, prob, y
+
+    whole = ask_rows(0, n)
+    assert bool((whole[0][:, 1] == 77).all())
+    for a, b in ((0, 700), (2 ** 25 - 300, 2 ** 25 + 300), (2 ** 26 - 300, 2 ** 26 + 300), (n - 900, n)):
+        assert all(torch.equal(u[a:b], v) for u, v in zip(whole, ask_rows(a, b)))
+    _, idx, prob, y = whole
+    assert bool((idx[:, 0] < 0).any()) and bool((idx[2 ** 26:, 1] >= 0).any())
+    prob.fill_(0.5)
+    dw, db, dy = torch.zeros(3, device=DEV), torch.zeros(3, device=DEV), torch.full((n, k), 77.0, device=DEV)
+    ws = torch.empty(s.mixture_grad_workspace(n, k), dtype=torch.uint8, device=DEV)
+    s.mixture_grad_dev(s.mixture_grad_args(n, k, x.data_ptr() + 4, idx.data_ptr(), prob.data_ptr(), y.data_ptr(), dout.data_ptr() + 8, dw.data_ptr(), db.data_ptr(), dy.data_ptr(),
+                                           x_row=2, dout_row=3, workspace=ws.data_ptr(), workspace_bytes=ws.numel(), stream=q))
+    torch.cuda.synchronize()
+    have = idx >= 0
+    assert torch.equal(dy, torch.where(have, 0.5 * dout[:, 2:], 0.0))
+    score = torch.where(have, y * dout[:, 2:], 0.0)
+    dl = torch.where(have, 0.5 * (score - 0.5 * score.sum(1, keepdim=True)), 0.0)
+    for e in range(3):
+        mine = torch.where(idx == e, dl, 0.0).sum(1, dtype=torch.float64)
+        assert dw[e].item() == np.float32((mine * x[:, 1]).sum().item()) and db[e].item() == np.float32(mine.sum().item())
